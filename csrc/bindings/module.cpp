@@ -474,6 +474,32 @@ PYBIND11_MODULE(_C, m) {
                                  seed.attr("__and__")(py::int_(0xFFFFFFFFFFFFFFFFull)).cast<uint64_t>());
   }, py::arg("qkv"), py::arg("heads"), py::arg("mask") = py::none(), py::arg("causal") = false, py::arg("scale") = 1.0,
      py::arg("dropout_p") = 0.0, py::arg("seed") = py::int_(0));
+  // Generation.
+  auto rotary_spec = [](const Tensor& turns, double magnitude, int64_t heads, bool interleaved, bool transposed) {
+    ops::RotarySpec s;
+    s.turns = turns; s.magnitude = magnitude; s.rotary_heads = heads; s.interleaved = interleaved; s.transposed = transposed;
+    return s;
+  };
+  m.def("_rotary_embedding", [rotary_spec](const Tensor& x, const py::object& pos, const Tensor& turns, double magnitude, int64_t heads,
+                                           bool interleaved, bool transposed) {
+    return ops::rotary_embedding(x, pos.is_none() ? Tensor() : pos.cast<Tensor>(), rotary_spec(turns, magnitude, heads, interleaved, transposed));
+  });
+  m.def("_rotary_embedding_", [rotary_spec](Tensor& x, const py::object& pos, const Tensor& turns, double magnitude, int64_t heads,
+                                            bool interleaved, bool transposed) {
+    return ops::rotary_embedding_(x, pos.is_none() ? Tensor() : pos.cast<Tensor>(), rotary_spec(turns, magnitude, heads, interleaved, transposed));
+  });
+  m.def("_paged_append_", [](Tensor& kp, Tensor& vp, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& starts, const py::object& counts) {
+    ops::paged_append_(kp, vp, k, v, table, starts, counts.is_none() ? Tensor() : counts.cast<Tensor>());
+  });
+  m.def("_copy_pages_", [](Tensor& pages, const std::vector<int64_t>& sources, const std::vector<int64_t>& destinations, int dim) {
+    ops::copy_pages_(pages, sources, destinations, dim);
+    return pages;
+  });
+  m.def("_paged_attention", &ops::paged_attention);
+  m.def("_beam_search_step", [](const Tensor& logits, const Tensor& scores, const py::object& finished, int64_t end_token) {
+    ops::BeamStep s = ops::beam_search_step(logits, scores, finished.is_none() ? Tensor() : finished.cast<Tensor>(), end_token);
+    return py::make_tuple(s.scores, s.parents, s.tokens, s.finished);
+  });
   // Diagnostics (reference project: bindings/ops_bindings.cpp:300-363, src/diagnostics/matmul.cpp).
   m.def("set_float32_matmul_precision", [](const std::string& level) {
     if (level == "highest") cu::set_float32_matmul_precision(0);

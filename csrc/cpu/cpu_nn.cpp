@@ -620,9 +620,11 @@ void sgd_cpu(OpCall& c) {
 }  // namespace
 
 void register_cpu_elementwise(KernelRegistry& r);
+void register_cpu_generation(KernelRegistry& r);
 
 void register_cpu_kernels(KernelRegistry& r) {
   register_cpu_elementwise(r);
+  register_cpu_generation(r);
   const uint8_t any = kContiguous | kStrided | kEmpty;
   const uint8_t packed = kContiguous | kEmpty;
 #define REG2(OP, FN, NAME, LAY)                                                                     \

@@ -1202,6 +1202,13 @@ unsigned int take_index_errors() {
   return host;
 }
 
+// The counter's address on the current device, for kernels of other files that bound indices.
+unsigned int* index_error_counter() {
+  void* p = nullptr;
+  OB_CUDA(cudaGetSymbolAddress(&p, g_index_errors));
+  return static_cast<unsigned int*>(p);
+}
+
 void register_cuda_nn(KernelRegistry& r) {
   const uint8_t packed = kContiguous | kEmpty;
 #define REG3(OP, FN, NAME)                                                                                      \

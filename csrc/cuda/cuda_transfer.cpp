@@ -15,6 +15,10 @@ void strided_copy_cuda(const Tensor& src, Tensor& dst, cudaStream_t st);
 void register_cuda_elementwise(KernelRegistry& r);
 void register_cuda_reduce(KernelRegistry& r);
 void register_cuda_nn(KernelRegistry& r);
+void register_cuda_rotary(KernelRegistry& r);
+void register_cuda_paged_cache(KernelRegistry& r);
+void register_cuda_paged_attention(KernelRegistry& r);
+void register_cuda_beam(KernelRegistry& r);
 void register_cuda_gemm(KernelRegistry& r);
 void register_cuda_conv(KernelRegistry& r);
 
@@ -116,6 +120,10 @@ void register_cuda_kernels(KernelRegistry& r) {
   cu::register_cuda_elementwise(r);
   cu::register_cuda_reduce(r);
   cu::register_cuda_nn(r);
+  cu::register_cuda_rotary(r);
+  cu::register_cuda_paged_cache(r);
+  cu::register_cuda_paged_attention(r);
+  cu::register_cuda_beam(r);
   cu::register_cuda_gemm(r);
   cu::register_cuda_conv(r);
 }

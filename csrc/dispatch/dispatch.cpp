@@ -161,6 +161,9 @@ KernelRegistry build_builtin_registry() {
   S(Fill, "fill_", 1, false); S(CopyRange, "copy_range", 2, false); S(ScatterSlice, "scatter_slice", 1, false);
   S(IsFiniteAll, "isfinite_all", 1, false); S(AmpUnscale, "amp_unscale", 1, false); S(AmpCopy, "amp_copy", 2, false);
   S(AdamStep, "adam_step", -1, false); S(SgdStep, "sgd_step", -1, false); S(BiasGrad, "bias_grad", 1, false);
+  S(RotaryEmbedding, "rotary_embedding", -1, false); S(PagedAppend, "paged_append_", -1, false);
+  S(CopyPages, "copy_pages_", 1, false); S(PagedAttention, "paged_attention", 5, false);
+  S(BeamSearchStep, "beam_search_step", -1, false);
 #undef S
   register_cpu_kernels(r);
   register_cuda_kernels(r);

@@ -107,6 +107,8 @@ inline void prefer_max_shared_carveout(Kernel kernel) {
 inline cudaStream_t stream_of(const OpCall& c) { return static_cast<cudaStream_t>(c.stream); }
 int sm_count_for(const Tensor& t);
 void check_launch(const char* what);
+// Device counter of indices that kernels found out of range (and did not follow).
+unsigned int* index_error_counter();
 
 struct Strided {
   int nd;

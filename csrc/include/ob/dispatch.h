@@ -32,6 +32,7 @@ enum class OperatorId : uint16_t {
   CausalSoftmax, CausalSoftmaxBackward,
   Cast, To, Contiguous, Fill, CopyRange, ScatterSlice,
   IsFiniteAll, AmpUnscale, AmpCopy, AdamStep, SgdStep, BiasGrad,
+  RotaryEmbedding, PagedAppend, CopyPages, PagedAttention, BeamSearchStep,
   COUNT
 };
 

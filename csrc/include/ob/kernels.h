@@ -39,7 +39,18 @@
 //  AmpCopy            in0=model(dst) in1=master(f32 src)
 //  AdamStep           in0=master in1=m in2=v in3=grad in4=model? f0=lr f1=b1 f2=b2 f3=eps f4=wd f5=bc1 f6=bc2 f7=grad_scale
 //  SgdStep            in0=master in1=grad in2=model? f0=lr f1=wd f2=grad_scale
+//  RotaryEmbedding    in0=x[B,T,H,D] (any strides, unit last) in1=positions(i32/i64 [T] or [B,T])? in2=turns per position
+//                     (f64 [R/2] on the host) out0=y (same shape; may be x itself) f0=sign f1=magnitude
+//                     i0=rotated heads i1=interleaved i2=in place (only turned values are written)
+//  PagedAppend        in0=k_pages in1=v_pages [N,H,P,D] (any page stride) in2=k in3=v [B,T,H,D] (unit last stride)
+//                     in4=page table i32 [B,M] in5=starts i32 [B] in6=counts i32 [B]?
+//  CopyPages          in0=pages (contiguous) i0=outer i1=pages i2=bytes of one page list=sources then destinations
+//  PagedAttention     in0=q [B,Hq,D] in1=k_pages in2=v_pages in3=page table i32 in4=lengths i32 out0=[B,Hq,D] f0=scale
+//  BeamSearchStep     in0=logits[B,W,V] in1=scores f32[B,W] in2=finished bool[B,W]? out0=scores f32 out1=parents i64
+//                     out2=tokens i64 out3=finished bool (all [B,W]) i0=end token (-1: none)
 #pragma once
+#include <math.h>
+
 #include "ob/dispatch.h"
 
 namespace ob {
@@ -52,6 +63,16 @@ inline bool extrema_better(T candidate, T best) {
   if (bn) return false;
   if (cn) return true;
   return candidate > best;
+}
+
+// Beams that offer the same scores tie, whatever order their exponentials were summed in: the
+// logarithm of the sum is rounded to 2^-30, far above the noise of the summation (about 2^-45) and
+// far below what scores are known to (2^-24 of their size).
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline double round_log_sum(double log_sum) {
+  return nearbyint(log_sum * 1073741824.0) * (1.0 / 1073741824.0);
 }
 
 // splitmix64 finalizer used by dropout on both backends; element i of a mask uses the

@@ -108,6 +108,39 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
 Tensor attention_packed(const Tensor& qkv, int64_t heads, const Tensor& mask, bool causal, double scale,
                         double dropout_p, uint64_t seed);
 
+// ---- generation
+// Turns pairs of values by position-dependent angles.  x: [B, T, H, D]; the first `rotary_heads`
+// heads have their first R values turned, everything else passes through.  `turns`: turns
+// (angle / 2 pi) per position of each of the R / 2 pairs, float64 on the host.  Pairs are (i, i + R/2), or (2i, 2i + 1)
+// with `interleaved`.  positions: undefined (0..T-1), [T] or [B, T].  `transposed` applies the
+// transposed map (negative angles), which is what carries a gradient back.
+struct RotarySpec {
+  Tensor turns;
+  double magnitude = 1.0;  // factor on the turned values
+  int64_t rotary_heads = 0;
+  bool interleaved = false, transposed = false;
+};
+Tensor rotary_embedding(const Tensor& x, const Tensor& positions, const RotarySpec& spec);
+Tensor& rotary_embedding_(Tensor& x, const Tensor& positions, const RotarySpec& spec);
+
+// Key-value cache in pages: k_pages / v_pages [N, H, P, D] hold P tokens of every head per page;
+// row b of `table` (int32 [B, M]) lists the pages of sequence b in order.  Writes k / v [B, T, H, D]:
+// token t < counts[b] (all T without counts) goes to place starts[b] + t of sequence b.
+void paged_append_(Tensor& k_pages, Tensor& v_pages, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& starts,
+                   const Tensor& counts);
+// pages[..., destinations[i], ...] = pages[..., sources[i], ...] along `dim`.  Destinations are
+// distinct and none of them is a source, so the order of the copies does not matter.
+void copy_pages_(Tensor& pages, const std::vector<int64_t>& sources, const std::vector<int64_t>& destinations, int dim);
+// Attention of one query per head, q [B, Hq, D], over the first lengths[b] cached tokens of each
+// sequence; query head h reads cached head h / (Hq / H).  A sequence of length 0 gives zeros.
+Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
+                       double scale);
+// One selection of beam search: see the definition at beam_search_step in functional.
+struct BeamStep {
+  Tensor scores, parents, tokens, finished;
+};
+BeamStep beam_search_step(const Tensor& logits, const Tensor& scores, const Tensor& finished, int64_t end_token);
+
 // ---- AMP / optimizer kernels
 std::pair<Tensor, bool> amp_unscale_to_f32_and_check(const Tensor& grad, double inv_scale);
 // Unscales into a new float32 tensor and ORs "saw a non-finite value" into `flag` (int32 [1]

@@ -89,6 +89,9 @@ def no_grad():
 
 
 from ._random import manual_seed  # noqa: E402,F401
+from .functional import (  # noqa: E402,F401
+    rotary_embedding, rotary_embedding_, paged_append_, copy_pages_, paged_attention, beam_search_step,
+)
 from . import functional, nn, optim, amp, training  # noqa: E402,F401
 from .checkpoint import (  # noqa: E402,F401
     save_state_dict, load_state_dict, save_checkpoint, load_checkpoint,

@@ -9,4 +9,5 @@ from .norm import LayerNorm, BatchNorm1d, BatchNorm2d  # noqa: F401
 from .embedding import Embedding  # noqa: F401
 from .loss import NLLLoss, CrossEntropyLoss  # noqa: F401
 from .attention import SelfAttention, MultiHeadSelfAttention  # noqa: F401
+from .rotary import RotaryEmbedding  # noqa: F401
 from .transformer import TransformerEncoderBlock  # noqa: F401

@@ -1,12 +1,35 @@
 // Attention of one new token over the paged key-value cache (sm_100a).
 //
-// o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q k_j - m),  m the running maximum, in one pass
-// over keys and values.
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(s_j - m),   s_j = log2(e) scale q k_j,   m = max_j s_j
+//
+// Keys and values are read once and the maximum runs along (a new one rescales what has been
+// summed), so the floor is the time that the cache's bytes take from HBM; about 4 H / H_kv
+// operations per cached value are far below what the tensor cores do in that time.
+//
+// Split.  The work is counted in slabs of 16 tokens of one cached head.  All slabs of the call, in
+// the order (sequence, head, token), are divided evenly over the warps of a persistent grid, whatever
+// the lengths are: a warp streams its own slabs and meets no other on the way.  A head that lies
+// within one warp's share is written at once; one that is spread leaves (m, sum p, sum p v) of each
+// share in a workspace, and a second kernel joins them in order.  It is launched as a dependent of
+// the first, so that its start-up hides behind it.  No atomics: the same call gives the same bits.
+//
+// Masks.  Rows behind a sequence's length are never read (they are zero-filled on the way in) and
+// weigh nothing; a score of -inf weighs nothing; NaN in what is seen stays NaN.
+#include <algorithm>
+#include <map>
+#include <mutex>
+#include <type_traits>
+#include <utility>
+
 #include "ob/cuda_common.cuh"
 
 namespace ob {
 namespace cu {
 namespace {
+
+constexpr int kSlab = 16;         // tokens
+constexpr int kMostBatch = 2048;  // sequences of one launch: their slab counts lie in shared memory
+constexpr int kMostWorkers = 4096;
 
 struct PagedArgs {
   const void *q, *k, *v;
@@ -14,105 +37,729 @@ struct PagedArgs {
   const int *table, *lengths;
   unsigned int* errors;
   long long qs[2], page_stride[2];  // batch and head of q; keys, values
-  int heads, kv_heads, head_dim, page_size, table_width, pages_total;
+  long long* prefix;                // workspace: slabs before each sequence, [batch + 1]
+  float2* stat;                     // workspace: (m, sum p) of [2 * workers][tile_heads]
+  float* part;                      // workspace: sum p v of [2 * workers][tile_heads][head_dim]
+  int batch, heads, kv_heads, head_dim, page_size, table_width, pages_total;
+  int tiles, tile_heads;            // query heads of one cached head are taken `tile_heads` at a time
+  int workers;
   float scale_log2;                 // scale * log2(e)
 };
 
-// Any type, head size and page size: a warp takes every fourth token, its lanes share the row.
-constexpr int kWarps = 4;
-template <class T, int PER_LANE>
-__global__ void __launch_bounds__(kWarps * 32) paged_rows_kernel(const __grid_constant__ PagedArgs a) {
-  __shared__ float part[kWarps][PER_LANE * 32 + 2];
-  const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads, kv = h / (a.heads / a.kv_heads);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.head_dim;
-  const long long most = a.pages_total > 0 ? static_cast<long long>(a.table_width) * a.page_size : 0;
-  long long n = a.lengths[b];
-  if (n < 0 || n > most) {
-    if (threadIdx.x == 0) atomicAdd(a.errors, 1u);
-    n = n < 0 ? 0 : most;
+__device__ __forceinline__ int length_of(const PagedArgs& a, int b) {
+  const int n = a.lengths[b];
+  const long long most = a.pages_total > 0 ? min(static_cast<long long>(a.table_width) * a.page_size, 2147483600LL) : 0;
+  return n < 0 ? 0 : n > most ? static_cast<int>(most) : n;
+}
+
+// A page number from the table; one out of range is counted and not followed.
+__device__ __forceinline__ int checked_page(const PagedArgs& a, int page, bool count) {
+  if (page >= 0 && page < a.pages_total) return page;
+  if (count) atomicAdd(a.errors, 1u);
+  return page < 0 ? 0 : a.pages_total - 1;
+}
+
+// Slabs before each sequence into shared memory; block 0 also leaves them for the joining kernel
+// and counts lengths that the table cannot hold.
+template <int THREADS>
+__device__ __forceinline__ void slab_prefix(const PagedArgs& a, long long* prefix) {
+  __shared__ long long warp_sum_[THREADS / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (a.batch + THREADS - 1) / THREADS, first = threadIdx.x * per, last = min(first + per, a.batch);
+  long long sum = 0;
+  for (int b = first; b < last; ++b) {
+    const int n = length_of(a, b);
+    if (blockIdx.x == 0 && n != a.lengths[b]) atomicAdd(a.errors, 1u);
+    sum += (n + kSlab - 1) / kSlab;
   }
-  const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[1];
-  float qv[PER_LANE], acc[PER_LANE], m = -INFINITY, l = 0.f;
+  long long run = sum;
 #pragma unroll
-  for (int i = 0; i < PER_LANE; ++i) {
-    const int d = i * 32 + lane;
-    qv[i] = d < D ? to_f(q[d]) * a.scale_log2 : 0.f;
-    acc[i] = 0.f;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += x;
   }
-  for (long long j = warp; j < n; j += kWarps) {
-    const long long slot = j / a.page_size;
-    int page = a.table[static_cast<long long>(b) * a.table_width + slot];
-    if (page < 0 || page >= a.pages_total) {
-      if (lane == 0) atomicAdd(a.errors, 1u);
-      page = page < 0 ? 0 : a.pages_total - 1;
-    }
-    const long long row = (static_cast<long long>(kv) * a.page_size + (j - slot * a.page_size)) * D;
-    const T* k = static_cast<const T*>(a.k) + page * a.page_stride[0] + row;
-    const T* v = static_cast<const T*>(a.v) + page * a.page_stride[1] + row;
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) {
-      const int d = i * 32 + lane;
-      if (d < D) dot = fmaf(qv[i], to_f(k[d]), dot);
-    }
-    dot = warp_sum(dot);
-    const float top = fmaxf(m, dot);
-    // A score of -inf weighs nothing whatever the maximum is so far; NaN stays NaN.
-    const float keep = m == top ? 1.f : exp2f(m - top), p = dot == -INFINITY ? 0.f : exp2f(dot - top);
-    l = l * keep + p;
-    m = top;
-#pragma unroll
-    for (int i = 0; i < PER_LANE; ++i) {
-      const int d = i * 32 + lane;
-      if (d < D) acc[i] = fmaf(p, to_f(v[d]), acc[i] * keep);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < PER_LANE; ++i) part[warp][i * 32 + lane] = acc[i];
-  if (lane == 0) { part[warp][PER_LANE * 32] = m; part[warp][PER_LANE * 32 + 1] = l; }
+  if (lane == 31) warp_sum_[warp] = run;
   __syncthreads();
-  float top = -INFINITY, sum = 0.f, w[kWarps];
-  for (int i = 0; i < kWarps; ++i) top = fmaxf(top, part[i][PER_LANE * 32]);
-  for (int i = 0; i < kWarps; ++i) {
-    w[i] = part[i][PER_LANE * 32] == top ? 1.f : exp2f(part[i][PER_LANE * 32] - top);
-    sum += w[i] * part[i][PER_LANE * 32 + 1];
+  long long before = run - sum;
+  for (int w = 0; w < warp; ++w) before += warp_sum_[w];
+  for (int b = first; b < last; ++b) {
+    prefix[b] = before;
+    if (blockIdx.x == 0) a.prefix[b] = before;
+    before += (length_of(a, b) + kSlab - 1) / kSlab;
+    if (b == a.batch - 1) {
+      prefix[a.batch] = before;
+      if (blockIdx.x == 0) a.prefix[a.batch] = before;
+    }
   }
+  __syncthreads();
+}
+
+// A place in the order of slabs.
+struct Cursor {
+  int b, item, j, slabs, n;  // sequence; (cached head, head tile); slab of it; slabs of it; length of the sequence
+  __device__ __forceinline__ void seek(const PagedArgs& a, const long long* prefix, int items, long long s) {
+    const long long u = s / items;
+    int lo = 0, hi = a.batch - 1;  // the last sequence whose prefix is <= u
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (prefix[mid] <= u) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    n = length_of(a, b);
+    slabs = static_cast<int>(prefix[b + 1] - prefix[b]);
+    const long long rest = s - prefix[b] * items;
+    item = static_cast<int>(rest / slabs);
+    j = static_cast<int>(rest - static_cast<long long>(item) * slabs);
+  }
+  // Not called behind the last slab of the call.
+  __device__ __forceinline__ void next(const PagedArgs& a, const long long* prefix, int items) {
+    if (++j < slabs) return;
+    j = 0;
+    if (++item < items) return;
+    item = 0;
+    do {
+      ++b;
+      slabs = static_cast<int>(prefix[b + 1] - prefix[b]);
+    } while (slabs == 0);
+    n = length_of(a, b);
+  }
+};
+
+// ------------------------------------------------------------- tensor-core warps
+// 16-bit types, head sizes that are a multiple of 8.  With K as the left operand a slab is one
+// m16n8k16 product per 16 values: S^T [16 tokens x 8 heads] = K q^T, and O^T [values x 8 heads]
+// += V^T P^T, so that up to 8 query heads of one cached head cost no more than one.  The weights
+// move from accumulator to operand layout by a transposing register move.  This product is far
+// from being the bound, and 8 columns is what a group of heads fills: tcgen05's tiles of 128 rows
+// would be empty.  Slabs arrive by asynchronous 16-byte copies into a ring of the warp's own.
+
+__device__ __forceinline__ void copy16(uint32_t smem, const void* global, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(global), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t smem) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
+}
+__device__ __forceinline__ void load_matrices_transposed(uint32_t (&r)[4], uint32_t smem) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <class T>
+__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  T v[2] = {from_f<T>(lo), from_f<T>(hi)};
+  return *reinterpret_cast<uint32_t*>(v);
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack2(const T* p) {
+  T v[2] = {p[0], p[1]};
+  return *reinterpret_cast<uint32_t*>(v);
+}
+
+template <int KD>
+struct SlabLayout {
+  static constexpr int kChunks = KD * 2;                            // 16-byte pieces of a row
+  static constexpr bool kSwizzled = (KD & (KD - 1)) == 0;           // else rows are padded by one piece
+  static constexpr int kPitch = KD * 32 + (kSwizzled ? 0 : 16);
+  static constexpr int kBytes = kSlab * kPitch;                     // keys or values of one slab
+  // Eight rows of the same piece lie in different banks.
+  __device__ static __forceinline__ uint32_t at(int row, int chunk) {
+    return static_cast<uint32_t>(row * kPitch + ((kSwizzled ? chunk ^ (row & 7) : chunk) << 4));
+  }
+};
+
+template <class T, int KD, int NT, int STAGES, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_constant__ PagedArgs a) {
+  using L = SlabLayout<KD>;
+  // Weights are at most 2^kLift: float16 then keeps full precision down to 2^-28 of the largest.
+  constexpr float kLift = std::is_same<T, __half>::value ? 14.f : 0.f;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  long long* prefix = reinterpret_cast<long long*>(smem + static_cast<size_t>(WARPS) * STAGES * 2 * L::kBytes);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  slab_prefix<WARPS * 32>(a, prefix);
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int items = a.kv_heads * a.tiles, D = a.head_dim, group = a.heads / a.kv_heads;
+  const long long total = prefix[a.batch] * items;
+  const long long workers = min(static_cast<long long>(a.workers), total);
+  const long long worker = static_cast<long long>(warp) * gridDim.x + blockIdx.x;  // few slabs spread over all SMs
+  if (worker >= workers) return;
+  const long long lo = total * worker / workers, hi = total * (worker + 1) / workers;
+
+  unsigned char* ring = smem + static_cast<size_t>(warp) * STAGES * 2 * L::kBytes;
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  const int real = D / 8;  // pieces of a row that exist; the others stay zero
+  if (real < L::kChunks) {
+    for (int i = lane; i < STAGES * 2 * kSlab * (L::kChunks - real); i += 32) {
+      const int row = i / (L::kChunks - real), chunk = real + i - row * (L::kChunks - real);
+      *reinterpret_cast<uint4*>(ring + (row / kSlab) * L::kBytes + L::at(row % kSlab, chunk)) = make_uint4(0, 0, 0, 0);
+    }
+    __syncwarp();
+  }
+  const bool whole_pages = a.page_size % kSlab == 0;  // then a slab lies within one page, its rows together
+  const int magic = (65536 + real - 1) / real;        // c / real for c < 512
+
+  Cursor ahead, now;
+  now.seek(a, prefix, items, lo);
+  ahead = now;
+  long long to_load = hi - lo;
+
+  auto page_at = [&](const Cursor& c) {
+    return whole_pages && to_load > 0
+               ? a.table[static_cast<long long>(c.b) * a.table_width + c.j * kSlab / a.page_size] : 0;
+  };
+  auto load_slab = [&](int stage, const Cursor& c, int page) {
+    const int n = c.n - c.j * kSlab;  // rows of the slab that exist
+    const int kv = c.item / a.tiles;
+    const uint32_t to = ring_at + stage * 2 * L::kBytes;
+    if (whole_pages) {
+      page = checked_page(a, page, lane == 0);
+      const long long inner = (static_cast<long long>(kv) * a.page_size + c.j * kSlab % a.page_size) * D;
+      const T* k = static_cast<const T*>(a.k) + page * a.page_stride[0] + inner;
+      const T* v = static_cast<const T*>(a.v) + page * a.page_stride[1] + inner;
+#pragma unroll
+      for (int i = 0; i < L::kChunks / 2; ++i) {
+        const int x = i * 32 + lane;
+        const int row = real == L::kChunks ? x / L::kChunks : (x * magic) >> 16;
+        if (row >= kSlab) break;
+        const uint32_t at = to + L::at(row, x - row * real);
+        const int bytes = row < n ? 16 : 0;
+        copy16(at, k + x * 8, bytes);
+        copy16(at + L::kBytes, v + x * 8, bytes);
+      }
+    } else {
+#pragma unroll 1
+      for (int x = lane; x < kSlab * real; x += 32) {
+        const int row = (x * magic) >> 16, chunk = x - row * real, token = c.j * kSlab + row;
+        const int slot = token / a.page_size;
+        const int entry = row < n ? a.table[static_cast<long long>(c.b) * a.table_width + slot] : 0;
+        const int pg = checked_page(a, entry, chunk == 0);
+        const long long inner = (static_cast<long long>(kv) * a.page_size + token - slot * a.page_size) * D + chunk * 8;
+        const uint32_t at = to + L::at(row, chunk);
+        const int bytes = row < n ? 16 : 0;
+        copy16(at, static_cast<const T*>(a.k) + (row < n ? pg * a.page_stride[0] + inner : 0), bytes);
+        copy16(at + L::kBytes, static_cast<const T*>(a.v) + (row < n ? pg * a.page_stride[1] + inner : 0), bytes);
+      }
+    }
+  };
+
+  int upcoming[STAGES - 1];  // page numbers first: their latencies overlap
+  {
+    Cursor c = ahead;
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+      upcoming[s] = s < to_load ? page_at(c) : 0;
+      if (s + 1 < to_load) c.next(a, prefix, items);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    if (to_load > 0) {
+      load_slab(s, ahead, upcoming[s]);
+      --to_load;
+      if (to_load > 0) ahead.next(a, prefix, items);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  int page = page_at(ahead);
+
+  uint32_t q[NT][KD][2];
+  float o[NT][KD][4], m[NT][2], sum[NT][2];
+  int stage = 0;
+  bool from_start = false, first_item = true;
+  // ldmatrix addresses: K rows are tokens, (0-7, 8-15) by lane bit 3, pieces by lane bit 4; V transposed, the other way round.
+  const int k_row = lane & 15, k_piece = lane >> 4, v_row = (lane & 7) + ((lane >> 4) << 3), v_piece = (lane >> 3) & 1;
+
+  for (long long left = hi - lo; left > 0; --left) {
+    const int kv = now.item / a.tiles, h0 = kv * group + (now.item - kv * a.tiles) * a.tile_heads;
+    const int heads = min(a.tile_heads, (kv + 1) * group - h0);
+    if (left == hi - lo || now.j == 0) {  // a new head: its queries, empty sums
+      from_start = now.j == 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const bool there = nt * 8 + g < heads;
+        const T* qh = static_cast<const T*>(a.q) + now.b * a.qs[0] + (h0 + nt * 8 + g) * a.qs[1];
+#pragma unroll
+        for (int i = 0; i < KD; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int d = i * 16 + e * 8 + t * 2;
+            q[nt][i][e] = there && d < D ? pack2<T>(qh + d) : 0u;
+          }
+#pragma unroll
+        for (int i = 0; i < KD; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+        m[nt][0] = m[nt][1] = -INFINITY;
+        sum[nt][0] = sum[nt][1] = 0.f;
+      }
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncwarp();  // every lane's copies are there, and every lane is done with the slab before
+    if (to_load > 0) {
+      load_slab(stage == 0 ? STAGES - 1 : stage - 1, ahead, page);
+      --to_load;
+      if (to_load > 0) ahead.next(a, prefix, items);
+      page = page_at(ahead);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+
+    const uint32_t ks = ring_at + stage * 2 * L::kBytes, vs = ks + L::kBytes;
+    float s[NT][4], s2[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KD; ++i) {
+      uint32_t k[4];
+      load_matrices(k, ks + L::at(k_row, i * 2 + k_piece));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) multiply<T>(i & 1 ? s2[nt] : s[nt], k, q[nt][i][0], q[nt][i][1]);  // two chains
+    }
+    uint32_t p[NT][2];
+    const int rows = now.n - now.j * kSlab;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      // s[0], s[1]: token g of heads 2t, 2t + 1; s[2], s[3]: token g + 8.
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[nt][e] = g + (e >> 1) * 8 < rows ? (s[nt][e] + s2[nt][e]) * a.scale_log2 : -INFINITY;
+      float top[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        top[c] = fmaxf(s[nt][c], s[nt][c + 2]);
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], x));
+        top[c] = fmaxf(top[c], m[nt][c]);
+      }
+      if (__any_sync(0xffffffffu, top[0] > m[nt][0] || top[1] > m[nt][1])) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float keep = top[c] == -INFINITY ? 1.f : exp2f(m[nt][c] - top[c]);
+          m[nt][c] = top[c];
+          sum[nt][c] *= keep;
+#pragma unroll
+          for (int i = 0; i < KD; ++i) {
+            o[nt][i][c] *= keep;
+            o[nt][i][c + 2] *= keep;
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float base = (m[nt][c] == -INFINITY ? 0.f : m[nt][c]) - kLift;
+        s[nt][c] = exp2f(s[nt][c] - base);
+        s[nt][c + 2] = exp2f(s[nt][c + 2] - base);
+        sum[nt][c] += s[nt][c] + s[nt][c + 2];
+      }
+      // The weights are rounded to the cache's type for the product with the values (half a step each).
+      p[nt][0] = transpose8x8(pack2<T>(s[nt][0], s[nt][1]));
+      p[nt][1] = transpose8x8(pack2<T>(s[nt][2], s[nt][3]));
+    }
+#pragma unroll
+    for (int i = 0; i < KD; ++i) {
+      uint32_t v[4];
+      load_matrices_transposed(v, vs + L::at(v_row, i * 2 + v_piece));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) multiply<T>(o[nt][i], v, p[nt][0], p[nt][1]);
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+
+    if (now.j == now.slabs - 1 || left == 1) {  // this share of the head is done
+      const bool all = from_start && now.j == now.slabs - 1;
+      const long long slot = (2 * worker + (first_item ? 0 : 1)) * a.tile_heads;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float w = sum[nt][c];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) w += __shfl_xor_sync(0xffffffffu, w, x);
+          const int h = nt * 8 + t * 2 + c;
+          if (h >= heads) continue;
+          if (all) {
+            T* out = static_cast<T*>(a.out) + (static_cast<long long>(now.b) * a.heads + h0 + h) * D;
+            const float inv = 1.f / w;
+#pragma unroll
+            for (int i = 0; i < KD; ++i) {
+              if (i * 16 + g < D) out[i * 16 + g] = from_f<T>(o[nt][i][c] * inv);
+              if (i * 16 + g + 8 < D) out[i * 16 + g + 8] = from_f<T>(o[nt][i][c + 2] * inv);
+            }
+          } else {
+            float* part = a.part + (slot + h) * D;
+            if (g == 0) a.stat[slot + h] = make_float2(m[nt][c], w);
+#pragma unroll
+            for (int i = 0; i < KD; ++i) {
+              if (i * 16 + g < D) part[i * 16 + g] = o[nt][i][c];
+              if (i * 16 + g + 8 < D) part[i * 16 + g + 8] = o[nt][i][c + 2];
+            }
+          }
+        }
+      first_item = false;
+    }
+    if (left > 1) now.next(a, prefix, items);
+  }
+}
+
+// ------------------------------------------------------------------- plain warps
+// float32, and head sizes or addresses that 16-byte pieces do not fit.  A lane holds PER values of
+// every row; 8 tokens are multiplied at a time with up to NH query heads, and their 8 NH partial
+// scores are summed over the lanes by halving: each exchange sends one half of the values and keeps
+// the other, so that a score costs about one exchange and ends in one lane, which takes its
+// exponential alone.
+template <class T, int PER>
+struct alignas(sizeof(T) * PER < 16 ? sizeof(T) * PER : 16) Row {
+  T v[PER];
+};
+
+template <class T, int PER>
+__device__ __forceinline__ Row<T, PER> load_row(const T* row, int d, int D, bool wide) {
+  Row<T, PER> r;
+  if (wide) {  // the head size and all addresses fit PER values
+    if (d < D) return *reinterpret_cast<const Row<T, PER>*>(row + d);
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) r.v[i] = !wide && d + i < D ? row[d + i] : from_f<T>(0.f);
+  return r;
+}
+
+// Sums of x[0..N) over the warp: the sum of x[i] ends in the lanes whose upper log2(N) bits are i.
+template <int N>
+__device__ __forceinline__ float sum_by_halving(float (&x)[N], int lane) {
+  int bit = 16;
+#pragma unroll
+  for (int n = N / 2; n > 0; n /= 2, bit /= 2) {
+    const bool upper = (lane & bit) != 0;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float keep = upper ? x[i + n] : x[i], send = upper ? x[i] : x[i + n];
+      x[i] = keep + __shfl_xor_sync(0xffffffffu, send, bit);
+    }
+  }
+  for (; bit > 0; bit /= 2) x[0] += __shfl_xor_sync(0xffffffffu, x[0], bit);
+  return x[0];
+}
+
+constexpr int kRowThreads = 256, kRowTokens = 8;
+template <class T, int PER, int NH>
+__global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_constant__ PagedArgs a, const bool wide) {
+  constexpr int kLaneHeads = NH < 4 ? NH : 4, kSets = NH / kLaneHeads;  // heads that the lanes hold side by side, and how often
+  constexpr int kShift = NH == 1 ? 2 : NH == 2 ? 1 : 0;                 // lane = (head, token, copy)
+  extern __shared__ __align__(16) long long rows_prefix[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  slab_prefix<kRowThreads>(a, rows_prefix);
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d0 = lane * PER;
+  const int items = a.kv_heads * a.tiles, D = a.head_dim, group = a.heads / a.kv_heads;
+  const int my_token = (lane >> kShift) & 7;
+  const long long total = rows_prefix[a.batch] * items;
+  const long long workers = min(static_cast<long long>(a.workers), total);
+  const long long worker = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
+  if (worker >= workers) return;
+  const long long lo = total * worker / workers, hi = total * (worker + 1) / workers;
+  Cursor now;
+  now.seek(a, rows_prefix, items, lo);
+
+  float q[NH][PER], acc[NH][PER], m[kSets], sum[kSets];
+  bool from_start = false, first_item = true;
+  for (long long left = hi - lo; left > 0; --left) {
+    const int kv = now.item / a.tiles, h0 = kv * group + (now.item - kv * a.tiles) * a.tile_heads;
+    const int heads = min(a.tile_heads, (kv + 1) * group - h0);
+    if (left == hi - lo || now.j == 0) {
+      from_start = now.j == 0;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const T* qh = static_cast<const T*>(a.q) + now.b * a.qs[0] + (h0 + h) * a.qs[1];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          q[h][i] = h < heads && d0 + i < D ? to_f(qh[d0 + i]) * a.scale_log2 : 0.f;
+          acc[h][i] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < kSets; ++c) { m[c] = -INFINITY; sum[c] = 0.f; }
+    }
+    const int* table = a.table + static_cast<long long>(now.b) * a.table_width;
+#pragma unroll 1
+    for (int first = now.j * kSlab; first < min(now.n, (now.j + 1) * kSlab); first += kRowTokens) {
+      const int rows = now.n - first;
+      Row<T, PER> k[kRowTokens], v[kRowTokens];
+      int slot = first / a.page_size, in_page = first - slot * a.page_size, page = checked_page(a, table[slot], lane == 0);
+#pragma unroll
+      for (int u = 0; u < kRowTokens; ++u) {
+        if (u < rows) {
+          if (in_page == a.page_size) {
+            in_page = 0;
+            page = checked_page(a, table[++slot], lane == 0);
+          }
+          const long long inner = (static_cast<long long>(kv) * a.page_size + in_page) * D;
+          k[u] = load_row<T, PER>(static_cast<const T*>(a.k) + page * a.page_stride[0] + inner, d0, D, wide);
+          v[u] = load_row<T, PER>(static_cast<const T*>(a.v) + page * a.page_stride[1] + inner, d0, D, wide);
+          ++in_page;
+        } else {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) k[u].v[i] = v[u].v[i] = from_f<T>(0.f);
+        }
+      }
+      float p[kSets];
+#pragma unroll
+      for (int c = 0; c < kSets; ++c) {
+        float x[kLaneHeads * kRowTokens];
+#pragma unroll
+        for (int h = 0; h < kLaneHeads; ++h)
+#pragma unroll
+          for (int u = 0; u < kRowTokens; ++u) {
+            float dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) dot = fmaf(q[c * kLaneHeads + h][i], to_f(k[u].v[i]), dot);
+            x[h * kRowTokens + u] = dot;
+          }
+        float s = sum_by_halving<kLaneHeads * kRowTokens>(x, lane);
+        s = my_token < rows ? s : -INFINITY;
+        float top = s;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o << kShift));
+        top = fmaxf(top, m[c]);
+        if (__any_sync(0xffffffffu, top > m[c])) {
+          const float keep = top == -INFINITY ? 1.f : exp2f(m[c] - top);
+          m[c] = top;
+          sum[c] *= keep;
+#pragma unroll
+          for (int h = 0; h < kLaneHeads; ++h) {
+            const float w = __shfl_sync(0xffffffffu, keep, h << (kShift + 3));
+#pragma unroll
+            for (int i = 0; i < PER; ++i) acc[c * kLaneHeads + h][i] *= w;
+          }
+        }
+        p[c] = exp2f(s - (m[c] == -INFINITY ? 0.f : m[c]));
+        sum[c] += p[c];
+      }
+#pragma unroll
+      for (int u = 0; u < kRowTokens; ++u)
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          const float w = __shfl_sync(0xffffffffu, p[h / kLaneHeads], ((h % kLaneHeads) << (kShift + 3)) | (u << kShift));
+#pragma unroll
+          for (int i = 0; i < PER; ++i) acc[h][i] = fmaf(w, to_f(v[u].v[i]), acc[h][i]);
+        }
+    }
+    if (now.j == now.slabs - 1 || left == 1) {
+      const bool all = from_start && now.j == now.slabs - 1;
+      const long long slot = (2 * worker + (first_item ? 0 : 1)) * a.tile_heads;
+#pragma unroll
+      for (int c = 0; c < kSets; ++c)
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], o << kShift);
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const float w = __shfl_sync(0xffffffffu, sum[h / kLaneHeads], (h % kLaneHeads) << (kShift + 3));
+        const float top = __shfl_sync(0xffffffffu, m[h / kLaneHeads], (h % kLaneHeads) << (kShift + 3));
+        if (h >= heads) continue;
+        if (!all && lane == 0) a.stat[slot + h] = make_float2(top, w);
+        T* out = static_cast<T*>(a.out) + (static_cast<long long>(now.b) * a.heads + h0 + h) * D;
+        float* part = a.part + (slot + h) * D;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (d0 + i < D) {
+            if (all) out[d0 + i] = from_f<T>(acc[h][i] / w);
+            else part[d0 + i] = acc[h][i];
+          }
+      }
+      first_item = false;
+    }
+    if (left > 1) now.next(a, rows_prefix, items);
+  }
+}
+
+// --------------------------------------------------------------------- joining
+// One block per sequence and query head: the shares of a head that was spread over several warps,
+// in their order, and zeros for an empty sequence.
+constexpr int kJoinThreads = 256;
+template <class T>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a) {
+  __shared__ float weight[kMostWorkers], smem[32], sums[kJoinThreads];
+  const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads, D = a.head_dim, tid = threadIdx.x;
+  const int group = a.heads / a.kv_heads, kv = h / group, tile = (h - kv * group) / a.tile_heads;
+  const int in_tile = h - kv * group - tile * a.tile_heads, items = a.kv_heads * a.tiles;
   T* out = static_cast<T*>(a.out) + static_cast<long long>(blockIdx.x) * D;
-  for (int d = threadIdx.x; d < D; d += kWarps * 32) {
-    float o = 0.f;
-    for (int i = 0; i < kWarps; ++i) o += w[i] * part[i][d];
-    out[d] = from_f<T>(n == 0 ? 0.f : o / sum);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long slabs = a.prefix[b + 1] - a.prefix[b];
+  if (slabs == 0) {
+    for (int d = tid; d < D; d += kJoinThreads) out[d] = from_f<T>(0.f);
+    return;
   }
+  const long long total = a.prefix[a.batch] * items, workers = min(static_cast<long long>(a.workers), total);
+  const long long s0 = a.prefix[b] * items + (kv * a.tiles + tile) * slabs, s1 = s0 + slabs;
+  // Worker c takes the slabs from total * c / workers on: the last one at or before s.
+  const long long first = ((s0 + 1) * workers - 1) / total, last = (s1 * workers - 1) / total;
+  if (first == last) return;  // its warp has written the result
+  const int n = static_cast<int>(last - first + 1);
+  // Only the first of them can have begun with another head.
+  const long long skipped = total * first / workers < s0 ? 1 : 0;
+  auto slot = [&](int c) { return (2 * (first + c) + (c == 0 ? skipped : 0)) * a.tile_heads + in_tile; };
+  float top = -INFINITY;
+  for (int c = tid; c < n; c += kJoinThreads) top = fmaxf(top, a.stat[slot(c)].x);
+  top = block_max(top, smem);
+  float sum = 0.f;
+  for (int c = tid; c < n; c += kJoinThreads) {
+    const float2 st = a.stat[slot(c)];
+    const float w = st.x == top ? 1.f : exp2f(st.x - top);
+    weight[c] = w;
+    sum += w * st.y;
+  }
+  sum = block_sum(sum, smem);  // synchronises: the weights are there
+  const int width = (D + 31) / 32 * 32, sides = kJoinThreads / width, side = tid / width, d = tid - side * width;
+  float o = 0.f;
+  if (side < sides && d < D)
+#pragma unroll 4
+    for (int c = side; c < n; c += sides) o = fmaf(weight[c], a.part[slot(c) * D + d], o);
+  sums[tid] = o;
+  __syncthreads();
+  if (side == 0 && d < D) {
+    for (int i = 1; i < sides; ++i) o += sums[i * width + d];
+    out[d] = from_f<T>(o / sum);
+  }
+}
+
+// ------------------------------------------------------------------------- host
+// Resident blocks per SM of a kernel with its shared memory, once per device; also opts in to it.
+template <class Kernel>
+int blocks_per_sm(Kernel kernel, int device, int threads, size_t smem) {
+  static std::mutex mu;  // one set per kernel type: the address tells the kernels apart
+  static std::map<std::pair<const void*, int>, int> known;
+  std::lock_guard<std::mutex> lock(mu);
+  int& n = known[{reinterpret_cast<const void*>(kernel), device}];
+  if (n == 0) {
+    OB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    int fit = 0;
+    OB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kernel, threads, smem));
+    if (fit < 1) throw std::runtime_error("paged_attention: the kernel does not fit this device");
+    n = fit;
+  }
+  return n;
+}
+
+struct Launch {
+  Device device;
+  int sms;
+  cudaStream_t stream;
+};
+
+// Both kernels of one call.  `smem_ring`: bytes in front of the slab counts.
+template <class T, class Kernel, class... Extra>
+void launch_both(Kernel kernel, int threads, size_t smem_ring, PagedArgs a, const Launch& l, Extra... extra) {
+  const int per_sm = blocks_per_sm(kernel, l.device.index, threads, smem_ring + (kMostBatch + 1) * sizeof(long long));
+  int blocks = l.sms * per_sm;
+  const int warps = threads / 32;
+  blocks = std::min(blocks, kMostWorkers / warps);
+  a.workers = blocks * warps;
+  const size_t shares = 2ull * a.workers * a.tile_heads;
+  const size_t prefix_bytes = (static_cast<size_t>(a.batch) * 8 + 8 + 255) / 256 * 256, stat_bytes = (shares * 8 + 255) / 256 * 256;
+  ScratchLease scratch(l.device, prefix_bytes + stat_bytes + shares * a.head_dim * 4, l.stream);
+  char* at = static_cast<char*>(scratch.data());
+  a.prefix = reinterpret_cast<long long*>(at);
+  a.stat = reinterpret_cast<float2*>(at + prefix_bytes);
+  a.part = reinterpret_cast<float*>(at + prefix_bytes + stat_bytes);
+  kernel<<<blocks, threads, smem_ring + (a.batch + 1) * sizeof(long long), l.stream>>>(a, extra...);
+  check_launch("paged_attention");
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(a.batch) * a.heads);
+  config.blockDim = dim3(kJoinThreads);
+  config.stream = l.stream;
+  cudaLaunchAttribute dependent{};
+  dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  dependent.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &dependent;
+  config.numAttrs = 1;
+  OB_CUDA(cudaLaunchKernelEx(&config, paged_join_kernel<T>, static_cast<const PagedArgs&>(a)));
+  check_launch("paged_attention join");
+}
+
+template <class T, int KD, int STAGES, int WARPS>
+void launch_tiles(PagedArgs a, const Launch& l) {
+  const int group = a.heads / a.kv_heads;
+  const int most = group <= 8 ? 8 : 16;
+  a.tiles = (group + most - 1) / most;
+  a.tile_heads = (group + a.tiles - 1) / a.tiles;
+  const size_t ring = static_cast<size_t>(WARPS) * STAGES * 2 * SlabLayout<KD>::kBytes;
+  if (most == 8) launch_both<T>(paged_tile_kernel<T, KD, 1, STAGES, WARPS>, WARPS * 32, ring, a, l);
+  else launch_both<T>(paged_tile_kernel<T, KD, 2, STAGES, WARPS>, WARPS * 32, ring, a, l);
+}
+
+template <class T, int PER>
+void launch_rows(PagedArgs a, const Launch& l, bool wide) {
+  const int group = a.heads / a.kv_heads;
+  const int most = PER == 8 ? 4 : 8;  // registers: queries and sums are NH x PER values each
+  a.tiles = (group + most - 1) / most;
+  a.tile_heads = (group + a.tiles - 1) / a.tiles;
+  if (a.tile_heads == 1) launch_both<T>(paged_rows_kernel<T, PER, 1>, kRowThreads, 0, a, l, wide);
+  else if (a.tile_heads == 2) launch_both<T>(paged_rows_kernel<T, PER, 2>, kRowThreads, 0, a, l, wide);
+  else if (a.tile_heads <= 4) launch_both<T>(paged_rows_kernel<T, PER, 4>, kRowThreads, 0, a, l, wide);
+  else if constexpr (PER < 8) launch_both<T>(paged_rows_kernel<T, PER, 8>, kRowThreads, 0, a, l, wide);
+}
+
+template <class T>
+void attend(const PagedArgs& a, const Launch& l) {
+  const long long strides = a.page_stride[0] | a.page_stride[1];
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
+  if constexpr (sizeof(T) == 2) {
+    if (a.head_dim % 8 == 0 && strides % 8 == 0 && bases % 16 == 0) {
+      if (a.head_dim <= 64) launch_tiles<T, 4, 6, 8>(a, l);
+      else if (a.head_dim <= 96) launch_tiles<T, 6, 4, 8>(a, l);
+      else if (a.head_dim <= 128) launch_tiles<T, 8, 3, 8>(a, l);
+      else launch_tiles<T, 16, 3, 4>(a, l);
+      return;
+    }
+  }
+  const int per = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8;
+  const bool wide = (a.head_dim | strides) % per == 0 && bases % std::min<size_t>(16, per * sizeof(T)) == 0;
+  if (per == 2) launch_rows<T, 2>(a, l, wide);
+  else if (per == 4) launch_rows<T, 4>(a, l, wide);
+  else launch_rows<T, 8>(a, l, wide);
 }
 
 template <class T>
 void k_paged_attention(OpCall& c) {
   const Tensor &q = c.in[0], &kp = c.in[1], &vp = c.in[2];
   const Shape& s = kp.shape();
-  const long long B = q.shape()[0], H = q.shape()[1];
-  if (B * H > 2147483647LL || s[0] > 2147483647LL || c.in[3].shape()[1] > 2147483647LL)
+  const long long B = q.shape()[0], H = q.shape()[1], width = c.in[3].shape()[1];
+  if (B * H > 2147483647LL || H * kMostBatch > 2147483647LL || s[0] > 2147483647LL || s[2] > 1073741823LL || width > 2147483647LL)
     throw std::invalid_argument("paged_attention: too many heads or pages");
   PagedArgs a{};
-  a.q = q.data(); a.k = kp.data(); a.v = vp.data(); a.out = c.out[0].data();
-  a.table = c.in[3].data_as<int>();
-  a.lengths = c.in[4].data_as<int>();
   a.errors = index_error_counter();
+  a.page_stride[0] = s[0] > 1 ? kp.strides()[0] : 0;
+  a.page_stride[1] = s[0] > 1 ? vp.strides()[0] : 0;
   for (int d = 0; d < 2; ++d) a.qs[d] = q.shape()[d] > 1 ? q.strides()[d] : 0;
-  a.page_stride[0] = kp.strides()[0];
-  a.page_stride[1] = vp.strides()[0];
+  a.k = kp.data();
+  a.v = vp.data();
   a.heads = static_cast<int>(H);
   a.kv_heads = static_cast<int>(s[1]);
   a.head_dim = static_cast<int>(s[3]);
   a.page_size = static_cast<int>(s[2]);
-  a.table_width = static_cast<int>(c.in[3].shape()[1]);
+  a.table_width = static_cast<int>(width);
   a.pages_total = static_cast<int>(s[0]);
   a.scale_log2 = static_cast<float>(c.f[0] * 1.4426950408889634);
-  const unsigned grid = static_cast<unsigned>(B * H);
-  cudaStream_t st = stream_of(c);
-  if (s[3] <= 64) paged_rows_kernel<T, 2><<<grid, kWarps * 32, 0, st>>>(a);
-  else if (s[3] <= 128) paged_rows_kernel<T, 4><<<grid, kWarps * 32, 0, st>>>(a);
-  else paged_rows_kernel<T, 8><<<grid, kWarps * 32, 0, st>>>(a);
-  check_launch("paged_attention");
+  const Launch l{q.device(), sm_count_for(q), stream_of(c)};
+  for (long long b = 0; b < B; b += kMostBatch) {
+    a.batch = static_cast<int>(std::min<long long>(kMostBatch, B - b));
+    a.q = q.data_as<T>() + b * a.qs[0];
+    a.out = c.out[0].data_as<T>() + b * H * s[3];
+    a.table = c.in[3].data_as<int>() + b * width;
+    a.lengths = c.in[4].data_as<int>() + b;
+    attend<T>(a, l);
+  }
 }
 
 }  // namespace

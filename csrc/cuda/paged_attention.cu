@@ -37,7 +37,6 @@ struct PagedArgs {
   const int *table, *lengths;
   unsigned int* errors;
   long long qs[2], page_stride[2];  // batch and head of q; keys, values
-  long long* prefix;                // workspace: slabs before each sequence, [batch + 1]
   float2* stat;                     // workspace: (m, sum p) of [2 * workers][tile_heads]
   float* part;                      // workspace: sum p v of [2 * workers][tile_heads][head_dim]
   int batch, heads, kv_heads, head_dim, page_size, table_width, pages_total;
@@ -52,6 +51,12 @@ __device__ __forceinline__ int length_of(const PagedArgs& a, int b) {
   return n < 0 ? 0 : n > most ? static_cast<int>(most) : n;
 }
 
+// Most quotients here fit 32 bits, where a division costs a fraction.
+__device__ __forceinline__ long long divide(long long x, long long y) {
+  if (((x | y) >> 32) == 0) return static_cast<unsigned>(x) / static_cast<unsigned>(y);
+  return x / y;
+}
+
 // A page number from the table; one out of range is counted and not followed.
 __device__ __forceinline__ int checked_page(const PagedArgs& a, int page, bool count) {
   if (page >= 0 && page < a.pages_total) return page;
@@ -59,17 +64,17 @@ __device__ __forceinline__ int checked_page(const PagedArgs& a, int page, bool c
   return page < 0 ? 0 : a.pages_total - 1;
 }
 
-// Slabs before each sequence into shared memory; block 0 also leaves them for the joining kernel
-// and counts lengths that the table cannot hold.
+// Slabs before each sequence into shared memory.  Returns the slabs of one warp's share: warp c of
+// the grid takes those from c * share on.
 template <int THREADS>
-__device__ __forceinline__ void slab_prefix(const PagedArgs& a, long long* prefix) {
+__device__ __forceinline__ long long slab_prefix(const PagedArgs& a, long long* prefix, bool count_errors) {
   __shared__ long long warp_sum_[THREADS / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (a.batch + THREADS - 1) / THREADS, first = threadIdx.x * per, last = min(first + per, a.batch);
   long long sum = 0;
   for (int b = first; b < last; ++b) {
     const int n = length_of(a, b);
-    if (blockIdx.x == 0 && n != a.lengths[b]) atomicAdd(a.errors, 1u);
+    if (count_errors && n != a.lengths[b]) atomicAdd(a.errors, 1u);
     sum += (n + kSlab - 1) / kSlab;
   }
   long long run = sum;
@@ -84,21 +89,18 @@ __device__ __forceinline__ void slab_prefix(const PagedArgs& a, long long* prefi
   for (int w = 0; w < warp; ++w) before += warp_sum_[w];
   for (int b = first; b < last; ++b) {
     prefix[b] = before;
-    if (blockIdx.x == 0) a.prefix[b] = before;
     before += (length_of(a, b) + kSlab - 1) / kSlab;
-    if (b == a.batch - 1) {
-      prefix[a.batch] = before;
-      if (blockIdx.x == 0) a.prefix[a.batch] = before;
-    }
+    if (b == a.batch - 1) prefix[a.batch] = before;
   }
   __syncthreads();
+  return divide(prefix[a.batch] * a.kv_heads * a.tiles + a.workers - 1, a.workers);
 }
 
 // A place in the order of slabs.
 struct Cursor {
   int b, item, j, slabs, n;  // sequence; (cached head, head tile); slab of it; slabs of it; length of the sequence
   __device__ __forceinline__ void seek(const PagedArgs& a, const long long* prefix, int items, long long s) {
-    const long long u = s / items;
+    const long long u = divide(s, items);
     int lo = 0, hi = a.batch - 1;  // the last sequence whose prefix is <= u
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -109,7 +111,7 @@ struct Cursor {
     n = length_of(a, b);
     slabs = static_cast<int>(prefix[b + 1] - prefix[b]);
     const long long rest = s - prefix[b] * items;
-    item = static_cast<int>(rest / slabs);
+    item = static_cast<int>(divide(rest, slabs));
     j = static_cast<int>(rest - static_cast<long long>(item) * slabs);
   }
   // Not called behind the last slab of the call.
@@ -164,11 +166,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   T v[2] = {from_f<T>(lo), from_f<T>(hi)};
   return *reinterpret_cast<uint32_t*>(v);
 }
-template <class T>
-__device__ __forceinline__ uint32_t pack2(const T* p) {
-  T v[2] = {p[0], p[1]};
-  return *reinterpret_cast<uint32_t*>(v);
-}
 
 template <int KD>
 struct SlabLayout {
@@ -190,15 +187,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
   extern __shared__ __align__(1024) unsigned char smem[];
   long long* prefix = reinterpret_cast<long long*>(smem + static_cast<size_t>(WARPS) * STAGES * 2 * L::kBytes);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  slab_prefix<WARPS * 32>(a, prefix);
+  const long long share = slab_prefix<WARPS * 32>(a, prefix, blockIdx.x == 0);
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int items = a.kv_heads * a.tiles, D = a.head_dim, group = a.heads / a.kv_heads;
   const long long total = prefix[a.batch] * items;
-  const long long workers = min(static_cast<long long>(a.workers), total);
   const long long worker = static_cast<long long>(warp) * gridDim.x + blockIdx.x;  // few slabs spread over all SMs
-  if (worker >= workers) return;
-  const long long lo = total * worker / workers, hi = total * (worker + 1) / workers;
+  const long long lo = worker * share, hi = min(lo + share, total);
+  if (lo >= hi) return;
 
   unsigned char* ring = smem + static_cast<size_t>(warp) * STAGES * 2 * L::kBytes;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
@@ -298,7 +294,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int d = i * 16 + e * 8 + t * 2;
-            q[nt][i][e] = there && d < D ? pack2<T>(qh + d) : 0u;
+            q[nt][i][e] = there && d < D ? *reinterpret_cast<const uint32_t*>(qh + d) : 0u;
           }
 #pragma unroll
         for (int i = 0; i < KD; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
@@ -459,16 +455,15 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
   constexpr int kShift = NH == 1 ? 2 : NH == 2 ? 1 : 0;                 // lane = (head, token, copy)
   extern __shared__ __align__(16) long long rows_prefix[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  slab_prefix<kRowThreads>(a, rows_prefix);
+  const long long share = slab_prefix<kRowThreads>(a, rows_prefix, blockIdx.x == 0);
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d0 = lane * PER;
   const int items = a.kv_heads * a.tiles, D = a.head_dim, group = a.heads / a.kv_heads;
   const int my_token = (lane >> kShift) & 7;
   const long long total = rows_prefix[a.batch] * items;
-  const long long workers = min(static_cast<long long>(a.workers), total);
   const long long worker = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
-  if (worker >= workers) return;
-  const long long lo = total * worker / workers, hi = total * (worker + 1) / workers;
+  const long long lo = worker * share, hi = min(lo + share, total);
+  if (lo >= hi) return;
   Cursor now;
   now.seek(a, rows_prefix, items, lo);
 
@@ -584,51 +579,114 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
 }
 
 // --------------------------------------------------------------------- joining
-// One block per sequence and query head: the shares of a head that was spread over several warps,
-// in their order, and zeros for an empty sequence.
-constexpr int kJoinThreads = 256;
+// The shares of a head that was spread over several warps, in their order; zeros for an empty
+// sequence.  What the shares are follows from the lengths alone and is worked out while the first
+// kernel still runs.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+
+struct Shares {
+  long long first_row, row0, step;  // rows of stat and part: share c > 0 at row0 + c * step
+  int n;                            // 0: an empty sequence; 1: nothing to join
+  __device__ __forceinline__ Shares(const PagedArgs& a, const long long* prefix, long long share, int b, int h) {
+    const int group = a.heads / a.kv_heads, kv = h / group, tile = (h - kv * group) / a.tile_heads;
+    const int in_tile = h - kv * group - tile * a.tile_heads;
+    const long long slabs = prefix[b + 1] - prefix[b];
+    n = 0;
+    first_row = row0 = 0;
+    step = 2 * a.tile_heads;
+    if (slabs == 0) return;
+    const long long s0 = prefix[b] * a.kv_heads * a.tiles + (kv * a.tiles + tile) * slabs;
+    const long long first = divide(s0, share);
+    n = static_cast<int>(divide(s0 + slabs - 1, share) - first) + 1;
+    row0 = first * step + in_tile;
+    // Only the first warp can have begun with another head: then this one is its second.
+    first_row = row0 + (first * share < s0 ? a.tile_heads : 0);
+  }
+  __device__ __forceinline__ long long row(int c) const { return c == 0 ? first_row : row0 + c * step; }
+};
+
+// Largest exponent and the sum that goes with it, over all shares; every lane gets both.
+__device__ __forceinline__ void join_stats(const PagedArgs& a, const Shares& s, int lane, float* top, float* sum) {
+  float m = -INFINITY, l = 0.f;
+  for (int c = lane; c < s.n; c += 32) {
+    const float2 st = a.stat[s.row(c)];
+    const float t = fmaxf(m, st.x);
+    l = l * (m == t ? 1.f : exp2f(m - t)) + st.y * (st.x == t ? 1.f : exp2f(st.x - t));
+    m = t;
+  }
+  *top = warp_max(m);
+  *sum = warp_sum(l * (m == *top ? 1.f : exp2f(m - *top)));
+}
+
+// Few heads with many shares: a block takes 32 values of one head, its warps every eighth share,
+// whose first loads are under way together with the maxima.
 template <class T>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a) {
-  __shared__ float weight[kMostWorkers], smem[32], sums[kJoinThreads];
-  const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads, D = a.head_dim, tid = threadIdx.x;
-  const int group = a.heads / a.kv_heads, kv = h / group, tile = (h - kv * group) / a.tile_heads;
-  const int in_tile = h - kv * group - tile * a.tile_heads, items = a.kv_heads * a.tiles;
+__global__ void __launch_bounds__(kJoinThreads) paged_join_wide_kernel(const __grid_constant__ PagedArgs a) {
+  constexpr int kAhead = 8;
+  extern __shared__ __align__(16) long long join_prefix[];
+  __shared__ float sums[kJoinWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.head_dim, d = blockIdx.y * 32 + lane;
+  const long long share = slab_prefix<kJoinThreads>(a, join_prefix, false);
+  const Shares s(a, join_prefix, share, blockIdx.x / a.heads, blockIdx.x % a.heads);
   T* out = static_cast<T*>(a.out) + static_cast<long long>(blockIdx.x) * D;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const long long slabs = a.prefix[b + 1] - a.prefix[b];
-  if (slabs == 0) {
-    for (int d = tid; d < D; d += kJoinThreads) out[d] = from_f<T>(0.f);
+  if (s.n < 2) {
+    if (s.n == 0 && warp == 0 && d < D) out[d] = from_f<T>(0.f);
     return;
   }
-  const long long total = a.prefix[a.batch] * items, workers = min(static_cast<long long>(a.workers), total);
-  const long long s0 = a.prefix[b] * items + (kv * a.tiles + tile) * slabs, s1 = s0 + slabs;
-  // Worker c takes the slabs from total * c / workers on: the last one at or before s.
-  const long long first = ((s0 + 1) * workers - 1) / total, last = (s1 * workers - 1) / total;
-  if (first == last) return;  // its warp has written the result
-  const int n = static_cast<int>(last - first + 1);
-  // Only the first of them can have begun with another head.
-  const long long skipped = total * first / workers < s0 ? 1 : 0;
-  auto slot = [&](int c) { return (2 * (first + c) + (c == 0 ? skipped : 0)) * a.tile_heads + in_tile; };
-  float top = -INFINITY;
-  for (int c = tid; c < n; c += kJoinThreads) top = fmaxf(top, a.stat[slot(c)].x);
-  top = block_max(top, smem);
-  float sum = 0.f;
-  for (int c = tid; c < n; c += kJoinThreads) {
-    const float2 st = a.stat[slot(c)];
-    const float w = st.x == top ? 1.f : exp2f(st.x - top);
-    weight[c] = w;
-    sum += w * st.y;
+  float x[kAhead], e[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int c = warp + i * kJoinWarps;
+    x[i] = c < s.n && d < D ? a.part[s.row(c) * D + d] : 0.f;
+    e[i] = c < s.n ? a.stat[s.row(c)].x : -INFINITY;
   }
-  sum = block_sum(sum, smem);  // synchronises: the weights are there
-  const int width = (D + 31) / 32 * 32, sides = kJoinThreads / width, side = tid / width, d = tid - side * width;
-  float o = 0.f;
-  if (side < sides && d < D)
-#pragma unroll 4
-    for (int c = side; c < n; c += sides) o = fmaf(weight[c], a.part[slot(c) * D + d], o);
-  sums[tid] = o;
+  float top, sum, o = 0.f;
+  join_stats(a, s, lane, &top, &sum);
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (warp + i * kJoinWarps < s.n) o = fmaf(e[i] == top ? 1.f : exp2f(e[i] - top), x[i], o);
+  if (d < D) {
+#pragma unroll 8
+    for (int c = warp + kAhead * kJoinWarps; c < s.n; c += kJoinWarps) {
+      const float ec = a.stat[s.row(c)].x;
+      o = fmaf(ec == top ? 1.f : exp2f(ec - top), a.part[s.row(c) * D + d], o);
+    }
+  }
+  sums[warp][lane] = o;
   __syncthreads();
-  if (side == 0 && d < D) {
-    for (int i = 1; i < sides; ++i) o += sums[i * width + d];
+  if (warp == 0 && d < D) {
+#pragma unroll
+    for (int i = 1; i < kJoinWarps; ++i) o += sums[i][lane];
+    out[d] = from_f<T>(o / sum);
+  }
+}
+
+// Many heads with few shares each: one warp per head.
+template <class T>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a) {
+  extern __shared__ __align__(16) long long join_prefix[];
+  const int lane = threadIdx.x & 31, D = a.head_dim;
+  const long long share = slab_prefix<kJoinThreads>(a, join_prefix, false);
+  const long long head = static_cast<long long>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
+  if (head >= static_cast<long long>(a.batch) * a.heads) return;
+  const Shares s(a, join_prefix, share, static_cast<int>(head) / a.heads, static_cast<int>(head) % a.heads);
+  T* out = static_cast<T*>(a.out) + head * D;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (s.n == 1) return;
+  if (s.n == 0) {
+    for (int d = lane; d < D; d += 32) out[d] = from_f<T>(0.f);
+    return;
+  }
+  float top, sum;
+  join_stats(a, s, lane, &top, &sum);
+  for (int d = lane; d < D; d += 32) {
+    float o = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < s.n; ++c) {
+      const float e = a.stat[s.row(c)].x;
+      o = fmaf(e == top ? 1.f : exp2f(e - top), a.part[s.row(c) * D + d], o);
+    }
     out[d] = from_f<T>(o / sum);
   }
 }
@@ -666,24 +724,25 @@ void launch_both(Kernel kernel, int threads, size_t smem_ring, PagedArgs a, cons
   blocks = std::min(blocks, kMostWorkers / warps);
   a.workers = blocks * warps;
   const size_t shares = 2ull * a.workers * a.tile_heads;
-  const size_t prefix_bytes = (static_cast<size_t>(a.batch) * 8 + 8 + 255) / 256 * 256, stat_bytes = (shares * 8 + 255) / 256 * 256;
-  ScratchLease scratch(l.device, prefix_bytes + stat_bytes + shares * a.head_dim * 4, l.stream);
-  char* at = static_cast<char*>(scratch.data());
-  a.prefix = reinterpret_cast<long long*>(at);
-  a.stat = reinterpret_cast<float2*>(at + prefix_bytes);
-  a.part = reinterpret_cast<float*>(at + prefix_bytes + stat_bytes);
+  const size_t stat_bytes = (shares * 8 + 255) / 256 * 256;
+  ScratchLease scratch(l.device, stat_bytes + shares * a.head_dim * 4, l.stream);
+  a.stat = static_cast<float2*>(scratch.data());
+  a.part = reinterpret_cast<float*>(static_cast<char*>(scratch.data()) + stat_bytes);
   kernel<<<blocks, threads, smem_ring + (a.batch + 1) * sizeof(long long), l.stream>>>(a, extra...);
   check_launch("paged_attention");
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(a.batch) * a.heads);
+  const unsigned heads = static_cast<unsigned>(a.batch) * a.heads, slices = static_cast<unsigned>((a.head_dim + 31) / 32);
+  const bool wide = heads * slices <= 4u * l.sms;
+  config.gridDim = wide ? dim3(heads, slices) : dim3((heads + kJoinWarps - 1) / kJoinWarps);
   config.blockDim = dim3(kJoinThreads);
+  config.dynamicSmemBytes = (a.batch + 1) * sizeof(long long);
   config.stream = l.stream;
   cudaLaunchAttribute dependent{};
   dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   dependent.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &dependent;
   config.numAttrs = 1;
-  OB_CUDA(cudaLaunchKernelEx(&config, paged_join_kernel<T>, static_cast<const PagedArgs&>(a)));
+  OB_CUDA(cudaLaunchKernelEx(&config, wide ? paged_join_wide_kernel<T> : paged_join_kernel<T>, static_cast<const PagedArgs&>(a)));
   check_launch("paged_attention join");
 }
 

@@ -243,7 +243,9 @@ Tensor paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_p
   Tensor out = Tensor::empty(q.shape(), q.dtype(), q.device());
   if (out.numel() == 0) return out;
   OpCall c;
+  // The kernels read queries in pairs: rows at odd places are copied (a few values next to the cache).
   c.in[0] = rows_of(q);
+  if (q.shape()[2] % 2 == 0 && (c.in[0].offset() | c.in[0].strides()[0] | c.in[0].strides()[1]) % 2 != 0) c.in[0] = clone(c.in[0]);
   c.in[1] = k_pages.detach();
   c.in[2] = v_pages.detach();
   c.in[3] = tab;

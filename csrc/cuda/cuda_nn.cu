@@ -8,6 +8,10 @@
 // composed LayerNorm / attention-softmax of python/orthon/nn/layernorm.py:34-61 and
 // python/orthon/functional/math.py:39-72.  Index errors never trap: out-of-range targets
 // are clamped and counted in a device error word the host can poll.
+#include <map>
+#include <mutex>
+#include <utility>
+
 #include "ob/cuda_common.cuh"
 #include "ob/ops.h"
 
@@ -1207,6 +1211,26 @@ unsigned int* index_error_counter() {
   void* p = nullptr;
   OB_CUDA(cudaGetSymbolAddress(&p, g_index_errors));
   return static_cast<unsigned int*>(p);
+}
+
+unsigned int* arrival_counters(Device dev, StreamHandle stream, size_t n) {
+  struct Counters {
+    Allocation memory;
+    size_t size = 0;
+  };
+  static std::mutex mu;
+  static auto* all = new std::map<std::pair<int, StreamHandle>, Counters>();  // as long as the memory pool
+  std::lock_guard<std::mutex> lock(mu);
+  Counters& c = (*all)[{dev.index, stream}];
+  if (c.size < n) {  // the smaller array goes back to the pool in stream order
+    size_t size = 4096;
+    while (size < n) size *= 2;
+    Allocation memory = MemoryPool::instance().acquire(dev, size * sizeof(unsigned int), stream);
+    OB_CUDA(cudaMemsetAsync(memory.data(), 0, size * sizeof(unsigned int), static_cast<cudaStream_t>(stream)));
+    c.memory = std::move(memory);
+    c.size = size;
+  }
+  return static_cast<unsigned int*>(c.memory.data());
 }
 
 void register_cuda_nn(KernelRegistry& r) {

@@ -4,7 +4,7 @@
 //
 // The logits are read once; that is the floor.  Within a beam the order of the candidates is the
 // order of the logits, so the beams are cut into chunks, and a warp takes from one its W best (value,
-// lowest place) together with its maximum and sum of exponentials, in one pass.  The last block of a
+// lowest place) together with its maximum and sum of exponentials, in one pass.  The last warp of a
 // sentence to arrive forms each beam's lse and picks the W best of the chunks' winners, in float64.
 //
 // One pass.  A warp's logits arrive by asynchronous copies, 128 pieces of 16 bytes at a time, into a
@@ -28,7 +28,7 @@ namespace ob {
 namespace cu {
 namespace {
 
-constexpr int kThreads = 128, kWarps = kThreads / 32, kBlocksPerSm = 5, kList = 1024;
+constexpr int kWarpsPerSm = 20, kMostLists = 256;  // blocks of one warp; chunks of a sentence that the selection has room for
 constexpr int kBatch = 4, kBatchVectors = kBatch * 32, kRing = 3, kStageBytes = (kBatchVectors + 1) * 16;
 constexpr int kAside = kBatchVectors + 32;  // pieces that a warp has room for: at least a batch at any time
 using Key = unsigned long long;  // order-preserving image of the value, then the complement of its place
@@ -79,6 +79,14 @@ __device__ __forceinline__ uint4 load16(const unsigned char* p, unsigned off) {
   }
 #undef OB_SHIFTED
   return r;
+}
+
+__device__ __forceinline__ Key order_of(double v) {
+  const Key u = static_cast<Key>(__double_as_longlong(v + 0.0));
+  return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double score_of(Key k) {
+  return __longlong_as_double(static_cast<long long>(k >> 63 ? k & 0x7fffffffffffffffull : ~k));
 }
 
 template <class T>
@@ -143,40 +151,49 @@ __device__ __forceinline__ Pair two(const Values<__nv_bfloat16>& x, int k) {
   return Pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// Smallest and largest of the maxima of `groups` groups of threads (thread modulo groups); every
-// thread gets both.  `shared`: 256 values.  Synchronises once.
-template <class F>
-__device__ __forceinline__ void group_maxima(F mine, int groups, F* shared, F* smallest, F* top) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, width = min(groups, 32);
-  for (int o = width; o < 32; o <<= 1) mine = fmax(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-  if (lane < width) shared[warp * width + lane] = mine;
-  __syncthreads();
-  F hi = static_cast<F>(-INFINITY), lo = static_cast<F>(INFINITY);
-  for (int g = lane; g < groups; g += 32) {  // 64 groups: two warps side by side
-    F m = static_cast<F>(-INFINITY);
-    for (int i = g; i < kWarps * width; i += groups) m = fmax(m, shared[i]);
-    hi = fmax(hi, m);
-    lo = fmin(lo, m);
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    hi = fmax(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    lo = fmin(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-  }
-  *smallest = lo;
-  *top = hi;
-}
-
-struct Shared {         // of the selection; it lies where the warps' memory was
-  double best[kList];
-  Key place[kList];     // (beam, token)
+struct Selection {      // of a sentence; it lies where the chunk's memory was
+  struct List {         // a chunk's winners that have not been taken yet
+    Key order, place;   // the first: order-preserving image of its score (0: none is left), (beam, token)
+    Key next;           // the second, as the chunk left it
+    double sum;         // of the chunk
+    float top;
+    int taken;          // entries behind the first two are found from here
+  } list[kMostLists];
   double base[64];      // score - lse, or the score of a finished beam; NaN: the beam offers nothing
-  float maxima[kThreads];
-  int count;
   bool ended[64];
 };
 
-// The W largest of keys[0..n) in order to sorted[0..W), zeros behind the last; by one warp.
-__device__ __forceinline__ void sort_best(const Key* keys, int n, Key* sorted, int W, int lane) {
+// The smallest of the maxima of `groups` interleaved groups of lanes; with 64 groups each lane has two.
+template <class K>
+__device__ __forceinline__ K least_maximum(K first, K second, int groups) {
+  K mine = groups <= 32 ? max(first, second) : min(first, second);
+  for (int o = groups; o < 32; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+  for (int o = 1; o < min(groups, 32); o <<= 1) mine = min(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+  return mine;
+}
+
+// The W largest of keys[0..n) in order to sorted[0..W), zeros behind the last; by one warp.  Each
+// counts the keys before it; when there are many, only those that reach the smallest of the
+// maxima of `groups` interleaved groups are left to count.
+__device__ __forceinline__ void sort_best(Key* keys, int n, Key* sorted, int W, int groups, int lane) {
+  if (n > 32 && n >= groups) {
+    Key first = 0, second = 0;
+    for (int i = lane; i < n; i += 64) {
+      first = max(first, keys[i]);
+      if (i + 32 < n) second = max(second, keys[i + 32]);
+    }
+    const Key mine = least_maximum(first, second, groups);
+    int left = 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const Key key = i0 + lane < n ? keys[i0 + lane] : 0;
+      const unsigned who = __ballot_sync(0xffffffffu, i0 + lane < n && key >= mine);
+      __syncwarp();
+      if (who >> lane & 1u) keys[left + __popc(who & ((1u << lane) - 1u))] = key;
+      left += __popc(who);
+    }
+    n = left;
+    __syncwarp();
+  }
   for (int i = n + lane; i < W; i += 32) sorted[i] = 0;
   for (int i = lane; i < n; i += 32) {
     const Key mine = keys[i];
@@ -194,10 +211,37 @@ __host__ __device__ constexpr size_t warp_bytes(int list) {
   return static_cast<size_t>(kRing) * kStageBytes + kAside * 20 + (static_cast<size_t>(list) + 64) * sizeof(Key);
 }
 
+// The W best of keys[0..held) and of the pieces' values above the bound, to sorted.
+template <class T>
+__device__ __noinline__ void take_one_by_one(const uint4* pieces, const int* numbers, int n, const Key* keys, int held, float bound, Key* sorted,
+                                             int W, int lane) {
+  constexpr int N = Values<T>::N;
+  Key after = ~0ull;
+  for (int r = 0; r < W; ++r) {
+    Key best = 0;
+    for (int i = lane; i < held; i += 32)
+      if (keys[i] < after && keys[i] > best) best = keys[i];
+    for (int i = lane; i < n; i += 32) {
+      const T* values = reinterpret_cast<const T*>(pieces + i);
+#pragma unroll 1
+      for (int k = 0; k < N; ++k) {
+        const float v = to_f(values[k]);
+        const Key key = make_key(v, numbers[i] * N + k);
+        if (v > bound && key < after && key > best) best = key;
+      }
+    }
+    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane == 0) sorted[r] = best;
+    after = best;
+  }
+  __syncwarp();
+}
+
 // The values of the pieces[0..n) that lie above the bound join the keys[0..held) chosen before; the W
 // best of all are left there, in order.  Returns how many there are.
 template <class T>
-__device__ __forceinline__ int cut(const uint4* pieces, const int* numbers, int n, Key* keys, int held, float bound, int list, int W, int lane) {
+__device__ __forceinline__ int cut(const uint4* pieces, const int* numbers, int n, Key* keys, int held, float bound, int list, int W, int groups,
+                                   int lane) {
   constexpr int N = Values<T>::N;
   Key* sorted = keys + list;
   __syncwarp();
@@ -205,47 +249,33 @@ __device__ __forceinline__ int cut(const uint4* pieces, const int* numbers, int 
   for (int i0 = 0; i0 < n; i0 += 32) {
     const bool there = i0 + lane < n;
     Values<T> x;
+    unsigned mine = 0;  // which of the piece's values count: hardly ever more than one
     int q = 0;
     if (there) {
       *reinterpret_cast<uint4*>(&x) = pieces[i0 + lane];
-      q = numbers[i0 + lane];
-    }
+      q = numbers[i0 + lane] * N;
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const float v = there ? to_f(x.v[k]) : -INFINITY;
-      const unsigned who = __ballot_sync(0xffffffffu, v > bound);
-      const int at = total + __popc(who & ((1u << lane) - 1u));
-      if (v > bound && at < list) keys[at] = make_key(v, q * N + k);
-      total += __popc(who);
+      for (int k = 0; k < N; ++k) mine |= to_f(x.v[k]) > bound ? 1u << k : 0u;
     }
+    const int many = __popc(mine);
+    int at = many;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int before = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += before;
+    }
+    const int all = __shfl_sync(0xffffffffu, at, 31);
+    at += total - many;
+    const T* values = reinterpret_cast<const T*>(pieces + i0 + lane);
+    for (; mine != 0; mine &= mine - 1, ++at) {
+      const int k = __ffs(mine) - 1;
+      if (at < list) keys[at] = make_key(to_f(values[k]), q + k);
+    }
+    total += all;
   }
   __syncwarp();
-  if (total <= list) {
-    sort_best(keys, total, sorted, W, lane);
-  } else {
-    Key after = ~0ull;
-    for (int r = 0; r < W; ++r) {
-      Key best = 0;
-      for (int i = lane; i < held; i += 32)
-        if (keys[i] < after && keys[i] > best) best = keys[i];
-      for (int i = lane; i < n; i += 32) {
-        Values<T> x;
-        *reinterpret_cast<uint4*>(&x) = pieces[i];
-        for (int k = 0; k < N; ++k) {
-          const float v = to_f(x.v[k]);
-          const Key key = make_key(v, numbers[i] * N + k);
-          if (v > bound && key < after && key > best) best = key;
-        }
-      }
-      for (int o = 16; o > 0; o >>= 1) {
-        const Key other = __shfl_xor_sync(0xffffffffu, best, o);
-        best = other > best ? other : best;
-      }
-      if (lane == 0) sorted[r] = best;
-      after = best;
-    }
-    __syncwarp();
-  }
+  if (total <= list) sort_best(keys, total, sorted, W, groups, lane);
+  else take_one_by_one<T>(pieces, numbers, n, keys, held, bound, sorted, W, lane);
   for (int i = lane; i < W; i += 32) keys[i] = sorted[i];
   __syncwarp();
   return min(total, W);
@@ -302,7 +332,7 @@ __device__ __forceinline__ void take_chunk(const T* __restrict__ logits, const B
   int stage = 0;
   for (int batch = 0;; ++batch) {
     if (batch == 1 || batch == batches || aside > kAside - kBatchVectors) {
-      held = cut<T>(pieces, numbers, aside, keys, held, bound, a.list, W, lane);
+      held = cut<T>(pieces, numbers, aside, keys, held, bound, a.list, W, a.groups, lane);
       // With W of them only a larger value can still displace one, for its place is behind theirs.
       bound = held == W ? key_value(keys[W - 1]) : -INFINITY;
       aside = 0;
@@ -313,19 +343,16 @@ __device__ __forceinline__ void take_chunk(const T* __restrict__ logits, const B
     if (batch + kRing - 1 < batches) load_batch(stage == 0 ? kRing - 1 : stage - 1);
     asm volatile("cp.async.commit_group;" ::: "memory");
     const int q0 = first + batch * kBatchVectors;
+    unsigned char* here = memory + stage * kStageBytes;
+    if (q0 + kBatchVectors > last || (q0 + kBatchVectors) * N > a.vocab) {  // what lies behind the chunk counts as -inf
+      T* values = reinterpret_cast<T*>(here + off);
+      for (int e = min(last * N, a.vocab) - q0 * N + lane; e < kBatchVectors * N; e += 32) values[e] = lowest<T>();
+      __syncwarp();
+    }
     Values<T> x[kBatch];
     float m[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) *reinterpret_cast<uint4*>(&x[i]) = load16(memory + stage * kStageBytes + (i * 32 + lane) * 16, off);
-    if (q0 + kBatchVectors > last || (q0 + kBatchVectors) * N > a.vocab) {
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-          const int q = q0 + i * 32 + lane;
-          if (q >= last || q * N + k >= a.vocab) x[i].v[k] = lowest<T>();
-        }
-    }
+    for (int i = 0; i < kBatch; ++i) *reinterpret_cast<uint4*>(&x[i]) = load16(here + (i * 32 + lane) * 16, off);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) m[i] = largest(x[i]);
     const float m01 = fmaxf(m[0], m[1]), m23 = fmaxf(m[2], m[3]), mine = fmaxf(m01, m23);
@@ -346,19 +373,14 @@ __device__ __forceinline__ void take_chunk(const T* __restrict__ logits, const B
       top = new_top;
     }
     if (batch == 0) {
-      float low = m01, high = m23;  // 64 groups: two of each lane
-      if (W <= 32) {
-        low = mine;
-        for (int o = a.groups; o < 32; o <<= 1) low = fmaxf(low, __shfl_xor_sync(0xffffffffu, low, o));
-        high = low;
-      }
-      low = -warp_max(-fminf(low, high));
+      const float low = least_maximum(m01, m23, a.groups);
       bound = low == -INFINITY ? low : nextafterf(low, -INFINITY);  // values that reach it lie above
     }
     if (__any_sync(0xffffffffu, mine > bound)) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const unsigned who = __ballot_sync(0xffffffffu, m[i] > bound);
+        if (who == 0) continue;
         if (m[i] > bound) {
           const int at = aside + __popc(who & ((1u << lane) - 1u));
           pieces[at] = *reinterpret_cast<const uint4*>(&x[i]);
@@ -391,162 +413,151 @@ __device__ __forceinline__ void take_chunk(const T* __restrict__ logits, const B
   for (int i = lane; i < W; i += 32) a.keys[slot * W + i] = keys[i];
 }
 
-// The selection of one sentence from its chunks' winners.
+// Entries n..W are -inf: the lowest places that have it.
 template <class T>
-__device__ __noinline__ void select_beams(const T* __restrict__ logits, const BeamArgs& a, int sentence, Shared& sh) {
-  const int W = a.beams, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__device__ __noinline__ void fill_up(const T* logits, const Selection* sh, float* scores, long long* parents, long long* tokens,
+                                     unsigned char* done, int n, int W, int vocab, int end) {
+  long long f = 0;
+  for (int k = n; k < W; ++f) {  // fewer than W places are passed over
+    const int w = static_cast<int>(f / vocab), v = static_cast<int>(f - static_cast<long long>(w) * vocab);
+    const bool nothing = isnan(sh->base[w]) || (sh->ended[w] ? v != end : !(to_f(logits[f]) > -INFINITY));
+    if (!nothing) continue;
+    scores[k] = -INFINITY;
+    parents[k] = w;
+    tokens[k] = v;
+    done[k++] = sh->ended[w] || v == end;
+  }
+}
+
+// The selection of one sentence from its chunks' winners; by one warp.  The chunks' lists are in
+// order: W times the best of their heads is taken, and its list moves on.  The warp comes here once
+// and finds the code in no instruction cache, so it is short loops rather than fast ones.
+template <class T>
+__device__ __forceinline__ void select_beams(const T* __restrict__ logits, const BeamArgs& a, int sentence, Selection& sh) {
+  const int W = a.beams, C = a.chunks, lane = threadIdx.x, lists = W * C;
   const long long row0 = static_cast<long long>(sentence) * W;
-  if (tid == 0) sh.count = 0;
-  for (int w = warp; w < W; w += kWarps) {
-    const float s = a.scores[row0 + w];
-    const bool fin = a.finished != nullptr && a.finished[row0 + w] != 0;
-    double b = s;
-    if (!isfinite(s)) b = NAN;
-    else if (!fin) {
-      const ChunkStat* st = a.stat + (row0 + w) * a.chunks;
-      float top = -INFINITY;
-      for (int c = lane; c < a.chunks; c += 32) top = fmaxf(top, __ldcg(&st[c].top));
-      top = warp_max(top);
-      double sum = 0.0;
-      for (int c = lane; c < a.chunks; c += 32) {
-        // A chunk without a finite value adds its sum (0, or NaN) as it is.
-        const float t = __ldcg(&st[c].top);
-        const double part = __ldcg(&st[c].sum);
-        sum += t == top || t == -INFINITY ? part : part * expf(t - top);
-      }
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      // log sum: the exponent in float64, the mantissa in [1, 2) in float32 (2^-24 either way).
-      int exponent;
-      const float mantissa = 2.f * frexpf(static_cast<float>(sum), &exponent);
-      b = top == -INFINITY || !isfinite(sum) ? static_cast<double>(NAN)
-                                             : s - (top + ((exponent - 1) * 0.69314718055994531 + static_cast<double>(logf(mantissa))));
-    }
-    if (lane == 0) {
-      sh.base[w] = b;
-      sh.ended[w] = fin;
-    }
-  }
-  __syncthreads();
-  const int per_row = a.chunks * W, n_all = W * per_row;  // candidates of a beam, of all
-  // Candidate i: its score, or -inf where there is none.
-  auto candidate = [&](int i, int w, Key* at) {
-    const double b = sh.base[w];
-    if (isnan(b)) return static_cast<double>(-INFINITY);
-    if (sh.ended[w]) {
-      *at = static_cast<Key>(w) << 32 | static_cast<unsigned>(a.end);
-      return i == w * per_row ? b : static_cast<double>(-INFINITY);
-    }
-    const Key key = __ldcg(a.keys + row0 * per_row + i);
-    if (key == 0) return static_cast<double>(-INFINITY);
-    *at = static_cast<Key>(w) << 32 | key_place(key);
-    return b + key_value(key);
-  };
-  // As in a chunk: the best of each chunk in G groups, the smallest of the groups' maxima as the
-  // bound.  Rounding down keeps the order, so that it can be done in float32.
-  float top = -INFINITY;
-  Key at = 0;
-  for (int i = tid; i < W * a.chunks; i += kThreads) top = fmaxf(top, __double2float_rd(candidate(i * W, i / a.chunks, &at)));
-  float reach, unused;
-  group_maxima<float>(top, a.groups, sh.maxima, &reach, &unused);
+  const Key* keys = a.keys + row0 * C * W;
 #pragma unroll 2
-  for (int i = tid; i < n_all; i += kThreads) {
-    const double c = candidate(i, i / per_row, &at);
-    if (c > -INFINITY && __double2float_rd(c) >= reach) {
-      const int to = atomicAdd(&sh.count, 1);
-      if (to < kList) {
-        sh.best[to] = c;
-        sh.place[to] = at;
-      }
-    }
+  for (int i = lane; i < lists; i += 32) {
+    const ChunkStat* st = a.stat + row0 * C + i;
+    const double sum = __ldcg(&st->sum);
+    const float top = __ldcg(&st->top);
+    const Key head = __ldcg(keys + i * W), next = W > 1 ? __ldcg(keys + i * W + 1) : 0;
+    Selection::List& l = sh.list[i];
+    l.sum = sum;
+    l.top = top;
+    l.order = head;
+    l.next = next;
+    l.taken = 2;
   }
-  __syncthreads();
-  const int n = sh.count;
-  auto emit = [&](int k, double score, int w, unsigned token) {
-    a.out_scores[row0 + k] = static_cast<float>(score);
-    a.parents[row0 + k] = w;
-    a.tokens[row0 + k] = token;
-    a.done[row0 + k] = sh.ended[w] || (a.end >= 0 && token == static_cast<unsigned>(a.end));
+  __syncwarp();
+#pragma unroll 1
+  for (int w = lane; w < W; w += 32) {
+    const float s = a.scores[row0 + w];
+    const bool ended = a.finished != nullptr && a.finished[row0 + w] != 0;
+    double base = isfinite(s) ? s : NAN;
+    Selection::List* l = sh.list + w * C;
+    if (!ended && isfinite(s)) {
+      float top = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < C; ++c) top = fmaxf(top, l[c].top);
+      double sum = 0.0;  // a chunk without a finite value adds its sum (0, or NaN) as it is
+#pragma unroll 1
+      for (int c = 0; c < C; ++c) sum += l[c].sum * (l[c].top == top || l[c].top == -INFINITY ? 1.f : __expf(l[c].top - top));
+      // log sum: the exponent in float64, the mantissa in [1, 2) in float32 (2^-24 either way).
+      const unsigned bits = __float_as_uint(static_cast<float>(sum));
+      const float mantissa = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
+      base = top == -INFINITY || !isfinite(sum)
+                 ? static_cast<double>(NAN)
+                 : s - (top + ((static_cast<int>(bits >> 23) - 127) * 0.69314718055994531 + static_cast<double>(logf(mantissa))));
+    }
+    sh.base[w] = base;
+    sh.ended[w] = ended;
+  }
+  __syncwarp();
+  // Heads become candidates.
+  auto offer = [&](Selection::List& l, int w, Key key, double base) {
+    l.order = key == 0 ? 0 : order_of(base + key_value(key));
+    l.place = static_cast<Key>(w) << 32 | key_place(key);
   };
-  if (n <= kList) {
-    for (int i = tid; i < n; i += kThreads) {
-      const double mine = sh.best[i];
-      const Key my_place = sh.place[i];
-      int before = 0;
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) before += sh.best[j] > mine || (sh.best[j] == mine && sh.place[j] < my_place);
-      if (before < W) emit(before, mine, static_cast<int>(my_place >> 32), static_cast<unsigned>(my_place));
+#pragma unroll 1
+  for (int i = lane; i < lists; i += 32) {
+    Selection::List& l = sh.list[i];
+    const int w = i / C;
+    const double base = sh.base[w];
+    if (isnan(base) || sh.ended[w]) {  // nothing, or a finished beam itself
+      l.order = !isnan(base) && i == w * C ? order_of(base) : 0;
+      l.place = static_cast<Key>(w) << 32 | static_cast<unsigned>(a.end);
+      l.next = 0;
+      l.taken = W;
+    } else {
+      offer(l, w, l.order, base);
     }
-    if (n < W && tid == 0) {  // nothing else is left than -inf: the lowest places that have it
-      const long long vocab = a.vocab;
-      long long f = 0;
-      for (int k = n; k < W; ++f) {  // fewer than W places are passed over
-        const int w = static_cast<int>(f / vocab);
-        const unsigned v = static_cast<unsigned>(f - w * vocab);
-        const bool nothing = isnan(sh.base[w]) ||
-                             (sh.ended[w] ? v != static_cast<unsigned>(a.end) : !(to_f(logits[row0 * vocab + f]) > -INFINITY));
-        if (nothing) emit(k++, -INFINITY, w, v);
-      }
-    }
-    return;
   }
-  double last = INFINITY;  // one by one, as above
-  Key last_at = 0;
-  for (int k = 0; k < W; ++k) {
-    double mine = -INFINITY;
-    Key my_place = ~0ull;
-    for (int i = tid; i < n_all; i += kThreads) {
-      const double c = candidate(i, i / per_row, &at);
-      if (c > -INFINITY && (c < last || (c == last && at > last_at)) && (c > mine || (c == mine && at < my_place))) {
-        mine = c;
-        my_place = at;
-      }
+  __syncwarp();
+  Key coming = 0;  // a list's entry on its way from memory; it is needed a round later at the earliest
+  int comes_to = -1, n = 0;
+#pragma unroll 1
+  for (; n < W; ++n) {
+    Key best = 0, place = ~0ull;
+    int from = -1;
+#pragma unroll 1
+    for (int i = lane; i < lists; i += 32) {
+      const Key o = sh.list[i].order, p = sh.list[i].place;
+      if (o > best || (o == best && o != 0 && p < place)) { best = o; place = p; from = i; }
     }
-    for (int o = 16; o > 0; o >>= 1) {
-      const double c = __shfl_xor_sync(0xffffffffu, mine, o);
-      const Key p = __shfl_xor_sync(0xffffffffu, my_place, o);
-      if (c > mine || (c == mine && p < my_place)) { mine = c; my_place = p; }
+    Key top = best, top_place = place;
+#pragma unroll 1
+    for (int x = 16; x > 0; x >>= 1) {
+      const Key o = __shfl_xor_sync(0xffffffffu, top, x), p = __shfl_xor_sync(0xffffffffu, top_place, x);
+      if (o > top || (o == top && p < top_place)) { top = o; top_place = p; }
     }
-    __syncthreads();
-    if (lane == 0) { sh.best[warp] = mine; sh.place[warp] = my_place; }
-    __syncthreads();
-    for (int w = 0; w < kWarps; ++w)
-      if (sh.best[w] > mine || (sh.best[w] == mine && sh.place[w] < my_place)) { mine = sh.best[w]; my_place = sh.place[w]; }
-    last = mine;
-    last_at = my_place;
-    if (tid == 0) emit(k, mine, static_cast<int>(my_place >> 32), static_cast<unsigned>(my_place));
+    if (top == 0) break;
+    if (best == top && place == top_place) {  // the lane that holds it
+      if (comes_to >= 0) sh.list[comes_to].next = coming;
+      const int w = static_cast<int>(top_place >> 32), token = static_cast<int>(static_cast<unsigned>(top_place));
+      a.out_scores[row0 + n] = static_cast<float>(score_of(top));
+      a.parents[row0 + n] = w;
+      a.tokens[row0 + n] = token;
+      a.done[row0 + n] = sh.ended[w] || token == a.end;
+      Selection::List& l = sh.list[from];
+      offer(l, w, l.next, sh.base[w]);
+      coming = l.taken < W ? __ldcg(keys + from * W + l.taken) : 0;
+      comes_to = from;
+      l.taken += 1;
+    }
+    __syncwarp();
   }
+  if (n < W && lane == 0)  // nothing else is left than -inf
+    fill_up<T>(logits + row0 * a.vocab, &sh, a.out_scores + row0, a.parents + row0, a.tokens + row0, a.done + row0, n, W, a.vocab, a.end);
 }
 
+// Blocks of one warp: chunks are uneven work (finished beams have none), and a warp that is done makes
+// room for the next at once.
 template <class T>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) beam_step_kernel(const T* __restrict__ logits, const __grid_constant__ BeamArgs a) {
+__global__ void __launch_bounds__(32, kWarpsPerSm) beam_step_kernel(const T* __restrict__ logits, const __grid_constant__ BeamArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ int flag;
-  const int warp = threadIdx.x >> 5, tasks = a.beams * a.chunks, blocks = (tasks + kWarps - 1) / kWarps;
-  const int sentence = blockIdx.x / blocks, task = (blockIdx.x - sentence * blocks) * kWarps + warp;
-  if (task < tasks) {
-    const int w = task / a.chunks;
-    const long long row = static_cast<long long>(sentence) * a.beams + w;
-    // A beam that has ended, or has no score, offers no continuation.
-    const bool ended = a.finished != nullptr && a.finished[row] != 0;
-    const float score = a.scores[row];
-    take_chunk<T>(logits, a, row, task - w * a.chunks, smem + warp * warp_bytes(a.list), [&] { return !ended && isfinite(score); });
-  }
-  if (last_to_arrive(a.arrived + sentence, static_cast<unsigned>(blocks), &flag))
-    select_beams<T>(logits, a, sentence, *reinterpret_cast<Shared*>(smem));
+  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, sentence = row / a.beams;
+  // A beam that has ended, or has no score, offers no continuation.
+  const bool ended = a.finished != nullptr && a.finished[row] != 0;
+  const float score = a.scores[row];
+  take_chunk<T>(logits, a, row, chunk, smem, [&] { return !ended && isfinite(score); });
+  if (last_warp_to_arrive(a.arrived + sentence, static_cast<unsigned>(a.beams) * a.chunks))
+    select_beams<T>(logits, a, sentence, *reinterpret_cast<Selection*>(smem));
 }
 
-// Chunks of a beam: enough warps for the device without chunks so short that their beginnings
-// and the joining cost more than they gain.  Both are counted in batches: a block's waves times
-// the batches of a chunk and four for its start (measured on one, 40 and 512 rows).
-int choose_chunks(long long sentences, int beams, long long vectors, int sms) {
-  const long long batches = (vectors + kBatchVectors - 1) / kBatchVectors;
-  long long best = 1, best_cost = 0;
-  for (long long c = 1; c <= std::min<long long>(batches, 256); ++c) {
-    const long long blocks = sentences * ((beams * c + kWarps - 1) / kWarps), slots = static_cast<long long>(sms) * kBlocksPerSm;
-    const long long cost = (blocks + slots - 1) / slots * ((batches + c - 1) / c + 4);
-    if (c == 1 || cost < best_cost) { best = c; best_cost = cost; }
+// Chunks of a beam.  In cycles: an SM that is full takes 82 for a batch (330 instructions of a warp), and a
+// chunk's start and end cost as many instructions as 6; a warp alone needs 900 for a batch.  The sum
+// of the two, everything at full rate and then one chunk to its end, is made small.
+int choose_chunks(long long rows, int beams, long long vectors, int sms) {
+  const double batches = static_cast<double>((vectors + kBatchVectors - 1) / kBatchVectors);
+  int best = 1;
+  double best_cost = 1e300;
+  for (int c = 1; c <= batches && c * beams <= kMostLists; ++c) {
+    const double cost = rows * (batches + 6.0 * c) * 82.0 / sms + (batches / c + 6.0) * 900.0;
+    if (cost < best_cost) { best = c; best_cost = cost; }
   }
-  return static_cast<int>(best);
+  return best;
 }
 
 template <class T>
@@ -554,7 +565,7 @@ void k_beam_step(OpCall& c) {
   const Shape& s = c.in[0].shape();
   constexpr int N = Values<T>::N;
   const long long rows = s[0] * s[1], vectors = (s[2] + N - 1) / N;
-  const long long chunks = choose_chunks(s[0], static_cast<int>(s[1]), vectors, sm_count_for(c.in[0]));
+  const long long chunks = choose_chunks(rows, static_cast<int>(s[1]), vectors, sm_count_for(c.in[0]));
   if (rows * chunks > 2147483647LL) throw std::invalid_argument("beam_search_step: too many rows");
   BeamArgs a{};
   a.scores = c.in[1].data_as<float>();
@@ -578,11 +589,9 @@ void k_beam_step(OpCall& c) {
   const T* logits = c.in[0].data_as<T>();
   a.arrived = arrival_counters(c.in[0].device(), st, static_cast<size_t>(s[0]));
   a.list = s[1] <= 8 ? 128 : s[1] <= 16 ? 256 : 512;
-  const size_t smem = kWarps * warp_bytes(a.list);
-  static_assert(sizeof(Shared) <= kWarps * warp_bytes(128), "the selection lies in the warps' memory");
-  OB_CUDA(cudaFuncSetAttribute(beam_step_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-  const long long blocks = s[0] * ((s[1] * chunks + kWarps - 1) / kWarps);
-  beam_step_kernel<T><<<static_cast<unsigned>(blocks), kThreads, smem, st>>>(logits, a);
+  const size_t smem = warp_bytes(a.list);
+  static_assert(sizeof(Selection) <= warp_bytes(128), "the selection lies in the chunk's memory");
+  beam_step_kernel<T><<<static_cast<unsigned>(rows * chunks), 32, smem, st>>>(logits, a);
   check_launch("beam_search_step");
 }
 

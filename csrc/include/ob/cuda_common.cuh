@@ -107,25 +107,23 @@ inline void prefer_max_shared_carveout(Kernel kernel) {
 inline cudaStream_t stream_of(const OpCall& c) { return static_cast<cudaStream_t>(c.stream); }
 int sm_count_for(const Tensor& t);
 void check_launch(const char* what);
-// Arrival counters for kernels whose last block finishes what the others left: `n` zeros that stay
+// Arrival counters for kernels whose last warp finishes what the others left: `n` zeros that stay
 // with the stream.  The last to arrive at a counter sets it back to zero, so that the next kernel on
 // the stream finds zeros again; kernels of one stream do not overlap.
 unsigned int* arrival_counters(Device dev, StreamHandle stream, size_t n);
 
-// Called by all threads of a block after they have written what the last block is to read: true in
-// the block that arrives last of `expected`.  What it reads then has to bypass the L1 cache
-// (__ldcg).  `flag`: a shared word.
-__device__ __forceinline__ bool last_to_arrive(unsigned int* counter, unsigned int expected, int* flag) {
-  __syncthreads();
-  if (threadIdx.x == 0) {  // the block's writes are ordered before its arrival by the barrier and this fence
+// Called by all lanes of a warp after they have written what the last warp is to read: true in the
+// warp that arrives last of `expected`.  What it reads then has to bypass the L1 cache (__ldcg).
+__device__ __forceinline__ bool last_warp_to_arrive(unsigned int* counter, unsigned int expected) {
+  __syncwarp();
+  int last = 0;
+  if ((threadIdx.x & 31) == 0) {  // the warp's writes are ordered before its arrival by the barrier and this fence
     __threadfence();
-    const bool last = atomicAdd(counter, 1u) == expected - 1;
+    last = atomicAdd(counter, 1u) == expected - 1;
     if (last) *counter = 0;
-    *flag = last;
     __threadfence();
   }
-  __syncthreads();
-  return *flag != 0;
+  return __shfl_sync(0xffffffffu, last, 0) != 0;
 }
 
 // Device counter of indices that kernels found out of range (and did not follow).

@@ -10,4 +10,5 @@ from .embedding import Embedding  # noqa: F401
 from .loss import NLLLoss, CrossEntropyLoss  # noqa: F401
 from .attention import SelfAttention, MultiHeadSelfAttention  # noqa: F401
 from .rotary import RotaryEmbedding  # noqa: F401
+from .kv_cache import PagedKVCache  # noqa: F401
 from .transformer import TransformerEncoderBlock  # noqa: F401

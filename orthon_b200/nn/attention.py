@@ -7,6 +7,7 @@ place through rank-4 tensor maps.
 from ..functional import scaled_dot_product_attention
 from .linear import Linear
 from .module import Module
+from .rotary import RotaryEmbedding
 
 
 class SelfAttention(Module):
@@ -32,7 +33,9 @@ class SelfAttention(Module):
 
 
 class MultiHeadSelfAttention(Module):
-    def __init__(self, embed_dim, num_heads, dropout=0.0):
+    """``rotary``: an `nn.RotaryEmbedding` that turns queries and keys by their positions 0..T-1."""
+
+    def __init__(self, embed_dim, num_heads, dropout=0.0, rotary=None):
         super().__init__()
         if embed_dim <= 0:
             raise ValueError("embed_dim must be positive")
@@ -43,6 +46,12 @@ class MultiHeadSelfAttention(Module):
         self.embed_dim, self.num_heads = int(embed_dim), int(num_heads)
         self.head_dim = self.embed_dim // self.num_heads
         self.dropout = float(dropout)
+        if rotary is not None:
+            if not isinstance(rotary, RotaryEmbedding):
+                raise TypeError("rotary must be a RotaryEmbedding or None")
+            if rotary.rotary_dim > self.head_dim:
+                raise ValueError("rotary_dim must not exceed the head size")
+        self.rotary = rotary
         self.q_proj = Linear(embed_dim, embed_dim)
         self.k_proj = Linear(embed_dim, embed_dim)
         self.v_proj = Linear(embed_dim, embed_dim)
@@ -55,8 +64,11 @@ class MultiHeadSelfAttention(Module):
         if E != self.embed_dim:
             raise ValueError(f"expected embed_dim={self.embed_dim}, got {E}")
         split = [B, T, self.num_heads, self.head_dim]
-        q = self.q_proj(x).reshape(split).transpose(1, 2)
-        k = self.k_proj(x).reshape(split).transpose(1, 2)
+        q = self.q_proj(x).reshape(split)
+        k = self.k_proj(x).reshape(split)
+        if self.rotary is not None:
+            q, k = self.rotary(q), self.rotary(k)
+        q, k = q.transpose(1, 2), k.transpose(1, 2)
         v = self.v_proj(x).reshape(split).transpose(1, 2)
         y = scaled_dot_product_attention(q, k, v, mask=mask, dropout_p=self.dropout, training=self.training,
                                          is_causal=is_causal)

@@ -16,7 +16,7 @@ constexpr int kThreads = 256;
 // ---------------------------------------------------------------------- append
 struct AppendArgs {
   char* pages[2];             // keys, values
-  const char* rows[2];
+  const char* rows_of[2];
   long long page_stride[2];   // in units (accesses of one thread)
   long long rs[2][3];         // batch, token, head strides of the rows, in units
   const int *table, *starts, *counts;
@@ -24,26 +24,56 @@ struct AppendArgs {
   int tokens, heads, page_size, units, table_width, pages_total;
 };
 
-// One block per token and side: the token's page is looked up once, then all heads are moved.
-template <class U>
+// A block takes TOKENS tokens of one sequence on one side.  Each thread keeps one access of one head;
+// its rows are fetched while other threads look up their places.  Heads with more accesses than a
+// block has threads go round again.
+template <class U, int TOKENS>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
-  const int b = blockIdx.x / a.tokens, t = blockIdx.x - b * a.tokens, side = blockIdx.y;
-  if (a.counts != nullptr && t >= a.counts[b]) return;
-  const long long at = static_cast<long long>(a.starts[b]) + t;
-  const long long slot = at / a.page_size;
-  int page = -1;
-  if (at >= 0 && slot < a.table_width) page = a.table[static_cast<long long>(b) * a.table_width + slot];
-  if (page < 0 || page >= a.pages_total) {  // never written: the row has no place
-    if (threadIdx.x == 0 && side == 0) atomicAdd(a.errors, 1u);
-    return;
+  __shared__ long long to[TOKENS];  // first access of the row's place, -1: not written
+  const int blocks = (a.tokens + TOKENS - 1) / TOKENS, b = blockIdx.x / blocks, t0 = (blockIdx.x - b * blocks) * TOKENS, side = blockIdx.y;
+  const int start = a.starts[b], count = a.counts == nullptr ? a.tokens : a.counts[b];
+  const int rows = min(min(TOKENS, a.tokens - t0), count - t0);
+  if (rows <= 0) return;
+  const int items = a.heads * a.units, i = threadIdx.x, h = i / a.units, u = i - h * a.units;
+  const U* src = reinterpret_cast<const U*>(a.rows_of[side]) + b * a.rs[side][0] + t0 * a.rs[side][1];
+  U* dst = reinterpret_cast<U*>(a.pages[side]);
+  const long long head_step = static_cast<long long>(a.page_size) * a.units;
+  U v[TOKENS];
+  if (i < items)
+#pragma unroll
+    for (int k = 0; k < TOKENS; ++k)
+      if (k < rows) v[k] = src[k * a.rs[side][1] + h * a.rs[side][2] + u];
+  if (i < rows) {
+    const long long at = static_cast<long long>(start) + t0 + i, slot = at / a.page_size;
+    int page = -1;
+    if (at >= 0 && slot < a.table_width) page = a.table[static_cast<long long>(b) * a.table_width + slot];
+    const bool there = page >= 0 && page < a.pages_total;
+    if (!there && side == 0) atomicAdd(a.errors, 1u);  // never written: the row has no place
+    to[i] = there ? page * a.page_stride[side] + (at - slot * a.page_size) * a.units : -1;
   }
-  U* dst = reinterpret_cast<U*>(a.pages[side]) + page * a.page_stride[side] + (at - slot * a.page_size) * a.units;
-  const U* src = reinterpret_cast<const U*>(a.rows[side]) + b * a.rs[side][0] + t * a.rs[side][1];
-  const int items = a.heads * a.units;
-  for (int i = threadIdx.x; i < items; i += kThreads) {
-    const int h = i / a.units, u = i - h * a.units;
-    dst[static_cast<long long>(h) * a.page_size * a.units + u] = src[h * a.rs[side][2] + u];
+  __syncthreads();
+  if (i < items)
+#pragma unroll
+    for (int k = 0; k < TOKENS; ++k)
+      if (k < rows && to[k] >= 0) dst[to[k] + h * head_step + u] = v[k];
+  for (int j = i + kThreads; j < items; j += kThreads) {
+    const int hj = j / a.units, uj = j - hj * a.units;
+#pragma unroll
+    for (int k = 0; k < TOKENS; ++k)
+      if (k < rows) v[k] = src[k * a.rs[side][1] + hj * a.rs[side][2] + uj];
+#pragma unroll
+    for (int k = 0; k < TOKENS; ++k)
+      if (k < rows && to[k] >= 0) dst[to[k] + hj * head_step + uj] = v[k];
   }
+}
+
+template <class U>
+void launch_append(const AppendArgs& a, long long batch, int sms, cudaStream_t st) {
+  // One token to a block until every SM has several blocks; then eight, whose loads are under way together.
+  const int tokens = batch * a.tokens >= 16ll * sms ? 8 : 1;
+  const dim3 grid(static_cast<unsigned>(batch * ((a.tokens + tokens - 1) / tokens)), 2);
+  if (tokens == 8) append_kernel<U, 8><<<grid, kThreads, 0, st>>>(a);
+  else append_kernel<U, 1><<<grid, kThreads, 0, st>>>(a);
 }
 
 // The widest of 16, 8, 4 and 2 bytes that divides every address, row and stride.
@@ -68,7 +98,7 @@ void k_paged_append(OpCall& c) {
   AppendArgs a{};
   for (int side = 0; side < 2; ++side) {
     a.pages[side] = c.in[side].data_as<char>();
-    a.rows[side] = c.in[2 + side].data_as<char>();
+    a.rows_of[side] = c.in[2 + side].data_as<char>();
     a.page_stride[side] = c.in[side].strides()[0] * size / w;
     for (int d = 0; d < 3; ++d) a.rs[side][d] = r[d] > 1 ? c.in[2 + side].strides()[d] * size / w : 0;
   }
@@ -82,12 +112,12 @@ void k_paged_append(OpCall& c) {
   a.units = static_cast<int>(row / w);
   a.table_width = static_cast<int>(c.in[4].shape()[1]);
   a.pages_total = static_cast<int>(s[0]);
-  const dim3 grid(static_cast<unsigned>(r[0] * r[1]), 2);
+  const int sms = sm_count_for(c.in[0]);
   cudaStream_t st = stream_of(c);
-  if (w == 16) append_kernel<uint4><<<grid, kThreads, 0, st>>>(a);
-  else if (w == 8) append_kernel<uint2><<<grid, kThreads, 0, st>>>(a);
-  else if (w == 4) append_kernel<unsigned int><<<grid, kThreads, 0, st>>>(a);
-  else append_kernel<unsigned short><<<grid, kThreads, 0, st>>>(a);
+  if (w == 16) launch_append<uint4>(a, r[0], sms, st);
+  else if (w == 8) launch_append<uint2>(a, r[0], sms, st);
+  else if (w == 4) launch_append<unsigned int>(a, r[0], sms, st);
+  else launch_append<unsigned short>(a, r[0], sms, st);
   check_launch("paged_append_");
 }
 

@@ -1208,9 +1208,18 @@ unsigned int take_index_errors() {
 
 // The counter's address on the current device, for kernels of other files that bound indices.
 unsigned int* index_error_counter() {
-  void* p = nullptr;
-  OB_CUDA(cudaGetSymbolAddress(&p, g_index_errors));
-  return static_cast<unsigned int*>(p);
+  static std::mutex mu;
+  static std::map<int, unsigned int*> known;  // asking the driver costs about as much as a launch
+  int device = 0;
+  OB_CUDA(cudaGetDevice(&device));
+  std::lock_guard<std::mutex> lock(mu);
+  unsigned int*& at = known[device];
+  if (at == nullptr) {
+    void* p = nullptr;
+    OB_CUDA(cudaGetSymbolAddress(&p, g_index_errors));
+    at = static_cast<unsigned int*>(p);
+  }
+  return at;
 }
 
 unsigned int* arrival_counters(Device dev, StreamHandle stream, size_t n) {

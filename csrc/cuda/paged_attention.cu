@@ -37,6 +37,7 @@ struct PagedArgs {
   const int *table, *lengths;
   unsigned int* errors;
   long long qs[2], page_stride[2];  // batch and head of q; keys, values
+  long long* prefix;                // workspace: slabs before each sequence, [batch + 1], and a warp's share
   float2* stat;                     // workspace: (m, sum p) of [2 * workers][tile_heads]
   float* part;                      // workspace: sum p v of [2 * workers][tile_heads][head_dim]
   int batch, heads, kv_heads, head_dim, page_size, table_width, pages_total;
@@ -64,69 +65,117 @@ __device__ __forceinline__ int checked_page(const PagedArgs& a, int page, bool c
   return page < 0 ? 0 : a.pages_total - 1;
 }
 
-// Slabs before each sequence into shared memory.  Returns the slabs of one warp's share: warp c of
-// the grid takes those from c * share on.
+__device__ __forceinline__ int slabs_of(int n) { return (n + kSlab - 1) / kSlab; }
+
+// A place in the order of slabs.  It moves on by counting: divisions cost more than the rest of a slab.
+struct Cursor {
+  int b, kv, tile;   // sequence, cached head, tile of its query heads
+  int j, slabs, n;   // slab of it; slabs of it; length of the sequence
+  int in_page;       // first token's place in its page, where pages are a multiple of slabs
+  // `rest`: slabs behind the first of sequence `at`.
+  __device__ __forceinline__ void set(const PagedArgs& a, int at, int length, long long rest) {
+    b = at;
+    n = length;
+    slabs = slabs_of(n);
+    const int item = static_cast<int>(divide(rest, slabs));
+    j = static_cast<int>(rest - static_cast<long long>(item) * slabs);
+    kv = item / a.tiles;
+    tile = item - kv * a.tiles;
+    in_page = j * kSlab % a.page_size;
+  }
+  // Not called behind the last slab of the call.
+  __device__ __forceinline__ void next(const PagedArgs& a) {
+    in_page += kSlab;
+    if (in_page >= a.page_size) in_page = 0;
+    if (++j < slabs) return;
+    j = in_page = 0;
+    if (++tile < a.tiles) return;
+    tile = 0;
+    if (++kv < a.kv_heads) return;
+    kv = 0;
+    do {
+      n = length_of(a, ++b);
+    } while (n == 0);
+    slabs = slabs_of(n);
+  }
+  __device__ __forceinline__ bool same_head(const Cursor& c) const { return b == c.b && kv == c.kv && tile == c.tile; }
+};
+
+// The share of this warp: warp c of the grid takes the slabs from c * share on.  Returns how many,
+// and the first of them in `at`.  Block 0 leaves the slabs before each sequence and the share for the
+// joining kernel and counts lengths that the table cannot hold.  Up to 32 sequences every warp counts
+// for itself; more are counted by the block, whose shared memory has room for their sums.
 template <int THREADS>
-__device__ __forceinline__ long long slab_prefix(const PagedArgs& a, long long* prefix, bool count_errors) {
-  __shared__ long long warp_sum_[THREADS / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = (a.batch + THREADS - 1) / THREADS, first = threadIdx.x * per, last = min(first + per, a.batch);
+__device__ __forceinline__ long long take_share(const PagedArgs& a, long long worker, long long* sums, Cursor* at) {
+  const int lane = threadIdx.x & 31, items = a.kv_heads * a.tiles;
+  const bool tell = blockIdx.x == 0;
+  long long all;  // slabs of one head
+  if (a.batch <= 32) {
+    const int n = lane < a.batch ? length_of(a, lane) : 0, mine = slabs_of(n);
+    if (tell && threadIdx.x < a.batch && n != a.lengths[lane]) atomicAdd(a.errors, 1u);
+    long long run = mine;
+#pragma unroll 1
+    for (int o = 1; o < a.batch; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += x;
+    }
+    all = __shfl_sync(0xffffffffu, run, a.batch - 1);
+    const long long share = divide(all * items + a.workers - 1, a.workers), lo = worker * share;
+    if (tell && threadIdx.x < a.batch) a.prefix[lane] = run - mine;
+    if (tell && threadIdx.x == 0) {
+      a.prefix[a.batch] = all;
+      a.prefix[a.batch + 1] = share;
+    }
+    if (lo >= all * items) return 0;
+    const long long u = divide(lo, items);
+    const int b = __popc(__ballot_sync(0xffffffffu, lane < a.batch && run <= u));
+    at->set(a, b, __shfl_sync(0xffffffffu, n, b), lo - __shfl_sync(0xffffffffu, run - mine, b) * items);
+    return min(share, all * items - lo);
+  }
+  __shared__ long long warp_sums[THREADS / 32];
+  const int warp = threadIdx.x >> 5, per = (a.batch + THREADS - 1) / THREADS, first = threadIdx.x * per, last = min(first + per, a.batch);
   long long sum = 0;
   for (int b = first; b < last; ++b) {
     const int n = length_of(a, b);
-    if (count_errors && n != a.lengths[b]) atomicAdd(a.errors, 1u);
-    sum += (n + kSlab - 1) / kSlab;
+    if (tell && n != a.lengths[b]) atomicAdd(a.errors, 1u);
+    sum += slabs_of(n);
   }
   long long run = sum;
-#pragma unroll
+#pragma unroll 1
   for (int o = 1; o < 32; o <<= 1) {
     const long long x = __shfl_up_sync(0xffffffffu, run, o);
     if (lane >= o) run += x;
   }
-  if (lane == 31) warp_sum_[warp] = run;
+  if (lane == 31) warp_sums[warp] = run;
   __syncthreads();
   long long before = run - sum;
-  for (int w = 0; w < warp; ++w) before += warp_sum_[w];
+  all = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    all += warp_sums[w];
+  }
   for (int b = first; b < last; ++b) {
-    prefix[b] = before;
-    before += (length_of(a, b) + kSlab - 1) / kSlab;
-    if (b == a.batch - 1) prefix[a.batch] = before;
+    sums[b] = before;
+    if (tell) a.prefix[b] = before;
+    before += slabs_of(length_of(a, b));
   }
   __syncthreads();
-  return divide(prefix[a.batch] * a.kv_heads * a.tiles + a.workers - 1, a.workers);
+  const long long share = divide(all * items + a.workers - 1, a.workers), lo = worker * share;
+  if (tell && threadIdx.x == 0) {
+    a.prefix[a.batch] = all;
+    a.prefix[a.batch + 1] = share;
+  }
+  if (lo >= all * items) return 0;
+  const long long u = divide(lo, items);
+  int low = 0, high = a.batch - 1;  // the last sequence with no more than u slabs before it
+  while (low < high) {
+    const int mid = (low + high + 1) >> 1;
+    if (sums[mid] <= u) low = mid;
+    else high = mid - 1;
+  }
+  at->set(a, low, length_of(a, low), lo - sums[low] * items);
+  return min(share, all * items - lo);
 }
-
-// A place in the order of slabs.
-struct Cursor {
-  int b, item, j, slabs, n;  // sequence; (cached head, head tile); slab of it; slabs of it; length of the sequence
-  __device__ __forceinline__ void seek(const PagedArgs& a, const long long* prefix, int items, long long s) {
-    const long long u = divide(s, items);
-    int lo = 0, hi = a.batch - 1;  // the last sequence whose prefix is <= u
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (prefix[mid] <= u) lo = mid;
-      else hi = mid - 1;
-    }
-    b = lo;
-    n = length_of(a, b);
-    slabs = static_cast<int>(prefix[b + 1] - prefix[b]);
-    const long long rest = s - prefix[b] * items;
-    item = static_cast<int>(divide(rest, slabs));
-    j = static_cast<int>(rest - static_cast<long long>(item) * slabs);
-  }
-  // Not called behind the last slab of the call.
-  __device__ __forceinline__ void next(const PagedArgs& a, const long long* prefix, int items) {
-    if (++j < slabs) return;
-    j = 0;
-    if (++item < items) return;
-    item = 0;
-    do {
-      ++b;
-      slabs = static_cast<int>(prefix[b + 1] - prefix[b]);
-    } while (slabs == 0);
-    n = length_of(a, b);
-  }
-};
 
 // ------------------------------------------------------------- tensor-core warps
 // 16-bit types, head sizes that are a multiple of 8.  With K as the left operand a slab is one
@@ -136,8 +185,11 @@ struct Cursor {
 // from being the bound, and 8 columns is what a group of heads fills: tcgen05's tiles of 128 rows
 // would be empty.  Slabs arrive by asynchronous 16-byte copies into a ring of the warp's own.
 
-__device__ __forceinline__ void copy16(uint32_t smem, const void* global, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(global), "r"(bytes) : "memory");
+__device__ __forceinline__ void copy16(uint32_t smem, const void* global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zero(uint32_t smem, const void* global, bool there) {  // nothing is read for a zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(global), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t smem) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -187,14 +239,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
   extern __shared__ __align__(1024) unsigned char smem[];
   long long* prefix = reinterpret_cast<long long*>(smem + static_cast<size_t>(WARPS) * STAGES * 2 * L::kBytes);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const long long share = slab_prefix<WARPS * 32>(a, prefix, blockIdx.x == 0);
-
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int items = a.kv_heads * a.tiles, D = a.head_dim, group = a.heads / a.kv_heads;
-  const long long total = prefix[a.batch] * items;
+  const int D = a.head_dim, group = a.heads / a.kv_heads;
   const long long worker = static_cast<long long>(warp) * gridDim.x + blockIdx.x;  // few slabs spread over all SMs
-  const long long lo = worker * share, hi = min(lo + share, total);
-  if (lo >= hi) return;
+  Cursor now;
+  const long long mine = take_share<WARPS * 32>(a, worker, prefix, &now);
+  if (mine == 0) return;
 
   unsigned char* ring = smem + static_cast<size_t>(warp) * STAGES * 2 * L::kBytes;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
@@ -209,33 +259,47 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
   const bool whole_pages = a.page_size % kSlab == 0;  // then a slab lies within one page, its rows together
   const int magic = (65536 + real - 1) / real;        // c / real for c < 512
 
-  Cursor ahead, now;
-  now.seek(a, prefix, items, lo);
-  ahead = now;
-  long long to_load = hi - lo;
+  Cursor ahead = now;
+  long long to_load = mine;
 
-  auto page_at = [&](const Cursor& c) {
-    return whole_pages && to_load > 0
-               ? a.table[static_cast<long long>(c.b) * a.table_width + c.j * kSlab / a.page_size] : 0;
+  // Page numbers of the next slabs of one head, one in each lane: fetched 32 at a time, because a
+  // load between the copies would wait for them.
+  int pages = 0, pages_from = 0, pages_b = -1;
+  auto page_of = [&](const Cursor& c) {
+    if (c.b != pages_b || c.j < pages_from || c.j >= pages_from + 32) {
+      pages_b = c.b;
+      pages_from = c.j;
+      const int j = c.j + lane;
+      pages = j < c.slabs ? a.table[static_cast<long long>(c.b) * a.table_width + j * kSlab / a.page_size] : 0;
+      if (j < c.slabs) pages = checked_page(a, pages, true);
+    }
+    return __shfl_sync(0xffffffffu, pages, c.j - pages_from);
   };
-  auto load_slab = [&](int stage, const Cursor& c, int page) {
+  const long long head_step = static_cast<long long>(a.page_size) * D;
+  auto load_slab = [&](int stage, const Cursor& c) {
     const int n = c.n - c.j * kSlab;  // rows of the slab that exist
-    const int kv = c.item / a.tiles;
     const uint32_t to = ring_at + stage * 2 * L::kBytes;
     if (whole_pages) {
-      page = checked_page(a, page, lane == 0);
-      const long long inner = (static_cast<long long>(kv) * a.page_size + c.j * kSlab % a.page_size) * D;
-      const T* k = static_cast<const T*>(a.k) + page * a.page_stride[0] + inner;
-      const T* v = static_cast<const T*>(a.v) + page * a.page_stride[1] + inner;
+      const int page = page_of(c);
+      const long long inner = c.kv * head_step + (c.in_page * D + lane * 8);
+      const T* k = static_cast<const T*>(a.k) + (page * a.page_stride[0] + inner);
+      const T* v = static_cast<const T*>(a.v) + (page * a.page_stride[1] + inner);
+      if (real == L::kChunks && n >= kSlab) {
 #pragma unroll
-      for (int i = 0; i < L::kChunks / 2; ++i) {
-        const int x = i * 32 + lane;
-        const int row = real == L::kChunks ? x / L::kChunks : (x * magic) >> 16;
-        if (row >= kSlab) break;
-        const uint32_t at = to + L::at(row, x - row * real);
-        const int bytes = row < n ? 16 : 0;
-        copy16(at, k + x * 8, bytes);
-        copy16(at + L::kBytes, v + x * 8, bytes);
+        for (int i = 0; i < L::kChunks / 2; ++i) {
+          const int x = i * 32 + lane;
+          const uint32_t at = to + L::at(x / L::kChunks, x % L::kChunks);
+          copy16(at, k + i * 256);
+          copy16(at + L::kBytes, v + i * 256);
+        }
+      } else {
+#pragma unroll 1
+        for (int x = lane; x < kSlab * real; x += 32, k += 256, v += 256) {
+          const int row = (x * magic) >> 16;
+          const uint32_t at = to + L::at(row, x - row * real);
+          copy16_or_zero(at, k, row < n);
+          copy16_or_zero(at + L::kBytes, v, row < n);
+        }
       }
     } else {
 #pragma unroll 1
@@ -244,58 +308,65 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
         const int slot = token / a.page_size;
         const int entry = row < n ? a.table[static_cast<long long>(c.b) * a.table_width + slot] : 0;
         const int pg = checked_page(a, entry, chunk == 0);
-        const long long inner = (static_cast<long long>(kv) * a.page_size + token - slot * a.page_size) * D + chunk * 8;
+        const long long inner = c.kv * head_step + (token - slot * a.page_size) * D + chunk * 8;
         const uint32_t at = to + L::at(row, chunk);
-        const int bytes = row < n ? 16 : 0;
-        copy16(at, static_cast<const T*>(a.k) + (row < n ? pg * a.page_stride[0] + inner : 0), bytes);
-        copy16(at + L::kBytes, static_cast<const T*>(a.v) + (row < n ? pg * a.page_stride[1] + inner : 0), bytes);
+        copy16_or_zero(at, static_cast<const T*>(a.k) + (row < n ? pg * a.page_stride[0] + inner : 0), row < n);
+        copy16_or_zero(at + L::kBytes, static_cast<const T*>(a.v) + (row < n ? pg * a.page_stride[1] + inner : 0), row < n);
       }
     }
   };
 
-  int upcoming[STAGES - 1];  // page numbers first: their latencies overlap
-  {
-    Cursor c = ahead;
+  constexpr bool kFetchAhead = KD * NT <= 16;  // as far as registers go
+  uint32_t q[NT][KD][2], coming[NT][KD][2];
+  Cursor whose = now;  // head that `coming` belongs to
+  bool fetched = false;
+  auto first_head = [&](const Cursor& c) { return c.kv * group + c.tile * a.tile_heads; };
+  auto heads_of = [&](const Cursor& c) { return min(a.tile_heads, group - c.tile * a.tile_heads); };
+  auto load_queries = [&](const Cursor& c, uint32_t (&to)[NT][KD][2]) {
+    const int h0 = first_head(c), heads = heads_of(c);
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-      upcoming[s] = s < to_load ? page_at(c) : 0;
-      if (s + 1 < to_load) c.next(a, prefix, items);
+    for (int nt = 0; nt < NT; ++nt) {
+      const bool there = nt * 8 + g < heads;
+      const T* qh = static_cast<const T*>(a.q) + c.b * a.qs[0] + (h0 + nt * 8 + g) * a.qs[1] + t * 2;
+#pragma unroll
+      for (int i = 0; i < KD; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          to[nt][i][e] = there && i * 16 + e * 8 + t * 2 < D ? *reinterpret_cast<const uint32_t*>(qh + i * 16 + e * 8) : 0u;
     }
-  }
-#pragma unroll
+  };
+  load_queries(now, q);
+#pragma unroll 1
   for (int s = 0; s < STAGES - 1; ++s) {
     if (to_load > 0) {
-      load_slab(s, ahead, upcoming[s]);
-      --to_load;
-      if (to_load > 0) ahead.next(a, prefix, items);
+      load_slab(s, ahead);
+      if (--to_load > 0) ahead.next(a);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
-  int page = page_at(ahead);
 
-  uint32_t q[NT][KD][2];
   float o[NT][KD][4], m[NT][2], sum[NT][2];
   int stage = 0;
   bool from_start = false, first_item = true;
   // ldmatrix addresses: K rows are tokens, (0-7, 8-15) by lane bit 3, pieces by lane bit 4; V transposed, the other way round.
   const int k_row = lane & 15, k_piece = lane >> 4, v_row = (lane & 7) + ((lane >> 4) << 3), v_piece = (lane >> 3) & 1;
 
-  for (long long left = hi - lo; left > 0; --left) {
-    const int kv = now.item / a.tiles, h0 = kv * group + (now.item - kv * a.tiles) * a.tile_heads;
-    const int heads = min(a.tile_heads, (kv + 1) * group - h0);
-    if (left == hi - lo || now.j == 0) {  // a new head: its queries, empty sums
+  for (long long left = mine; left > 0; --left) {
+    if (left == mine || now.j == 0) {  // a new head: its queries, empty sums
       from_start = now.j == 0;
+      if (left != mine) {
+        if (!kFetchAhead || !fetched || !whose.same_head(now)) load_queries(now, coming);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < KD; ++i) {
+            q[nt][i][0] = coming[nt][i][0];
+            q[nt][i][1] = coming[nt][i][1];
+          }
+        fetched = false;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const bool there = nt * 8 + g < heads;
-        const T* qh = static_cast<const T*>(a.q) + now.b * a.qs[0] + (h0 + nt * 8 + g) * a.qs[1];
-#pragma unroll
-        for (int i = 0; i < KD; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int d = i * 16 + e * 8 + t * 2;
-            q[nt][i][e] = there && d < D ? *reinterpret_cast<const uint32_t*>(qh + d) : 0u;
-          }
 #pragma unroll
         for (int i = 0; i < KD; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
         m[nt][0] = m[nt][1] = -INFINITY;
@@ -305,10 +376,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();  // every lane's copies are there, and every lane is done with the slab before
     if (to_load > 0) {
-      load_slab(stage == 0 ? STAGES - 1 : stage - 1, ahead, page);
-      --to_load;
-      if (to_load > 0) ahead.next(a, prefix, items);
-      page = page_at(ahead);
+      load_slab(stage == 0 ? STAGES - 1 : stage - 1, ahead);
+      if (--to_load > 0) {
+        ahead.next(a);
+        if (kFetchAhead && ahead.j == 0 && !fetched) {  // the next head's queries, while this one's slabs are taken
+          load_queries(ahead, coming);
+          whose = ahead;
+          fetched = true;
+        }
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 
@@ -375,6 +451,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
 
     if (now.j == now.slabs - 1 || left == 1) {  // this share of the head is done
       const bool all = from_start && now.j == now.slabs - 1;
+      const int h0 = first_head(now), heads = heads_of(now);
       const long long slot = (2 * worker + (first_item ? 0 : 1)) * a.tile_heads;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -405,7 +482,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
         }
       first_item = false;
     }
-    if (left > 1) now.next(a, prefix, items);
+    if (left > 1) now.next(a);
   }
 }
 
@@ -455,24 +532,19 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
   constexpr int kShift = NH == 1 ? 2 : NH == 2 ? 1 : 0;                 // lane = (head, token, copy)
   extern __shared__ __align__(16) long long rows_prefix[];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const long long share = slab_prefix<kRowThreads>(a, rows_prefix, blockIdx.x == 0);
-
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d0 = lane * PER;
-  const int items = a.kv_heads * a.tiles, D = a.head_dim, group = a.heads / a.kv_heads;
+  const int D = a.head_dim, group = a.heads / a.kv_heads;
   const int my_token = (lane >> kShift) & 7;
-  const long long total = rows_prefix[a.batch] * items;
   const long long worker = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
-  const long long lo = worker * share, hi = min(lo + share, total);
-  if (lo >= hi) return;
   Cursor now;
-  now.seek(a, rows_prefix, items, lo);
+  const long long mine = take_share<kRowThreads>(a, worker, rows_prefix, &now);
+  if (mine == 0) return;
 
   float q[NH][PER], acc[NH][PER], m[kSets], sum[kSets];
   bool from_start = false, first_item = true;
-  for (long long left = hi - lo; left > 0; --left) {
-    const int kv = now.item / a.tiles, h0 = kv * group + (now.item - kv * a.tiles) * a.tile_heads;
-    const int heads = min(a.tile_heads, (kv + 1) * group - h0);
-    if (left == hi - lo || now.j == 0) {
+  for (long long left = mine; left > 0; --left) {
+    const int h0 = now.kv * group + now.tile * a.tile_heads, heads = min(a.tile_heads, group - now.tile * a.tile_heads);
+    if (left == mine || now.j == 0) {
       from_start = now.j == 0;
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
@@ -499,7 +571,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
             in_page = 0;
             page = checked_page(a, table[++slot], lane == 0);
           }
-          const long long inner = (static_cast<long long>(kv) * a.page_size + in_page) * D;
+          const long long inner = (static_cast<long long>(now.kv) * a.page_size + in_page) * D;
           k[u] = load_row<T, PER>(static_cast<const T*>(a.k) + page * a.page_stride[0] + inner, d0, D, wide);
           v[u] = load_row<T, PER>(static_cast<const T*>(a.v) + page * a.page_stride[1] + inner, d0, D, wide);
           ++in_page;
@@ -574,28 +646,27 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
       }
       first_item = false;
     }
-    if (left > 1) now.next(a, rows_prefix, items);
+    if (left > 1) now.next(a);
   }
 }
 
 // --------------------------------------------------------------------- joining
 // The shares of a head that was spread over several warps, in their order; zeros for an empty
-// sequence.  What the shares are follows from the lengths alone and is worked out while the first
-// kernel still runs.
+// sequence.
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
 
 struct Shares {
   long long first_row, row0, step;  // rows of stat and part: share c > 0 at row0 + c * step
   int n;                            // 0: an empty sequence; 1: nothing to join
-  __device__ __forceinline__ Shares(const PagedArgs& a, const long long* prefix, long long share, int b, int h) {
+  __device__ __forceinline__ Shares(const PagedArgs& a, int b, int h) {
+    const long long before = __ldcg(a.prefix + b), slabs = __ldcg(a.prefix + b + 1) - before, share = __ldcg(a.prefix + a.batch + 1);
     const int group = a.heads / a.kv_heads, kv = h / group, tile = (h - kv * group) / a.tile_heads;
     const int in_tile = h - kv * group - tile * a.tile_heads;
-    const long long slabs = prefix[b + 1] - prefix[b];
     n = 0;
     first_row = row0 = 0;
     step = 2 * a.tile_heads;
     if (slabs == 0) return;
-    const long long s0 = prefix[b] * a.kv_heads * a.tiles + (kv * a.tiles + tile) * slabs;
+    const long long s0 = before * a.kv_heads * a.tiles + (kv * a.tiles + tile) * slabs;
     const long long first = divide(s0, share);
     n = static_cast<int>(divide(s0 + slabs - 1, share) - first) + 1;
     row0 = first * step + in_tile;
@@ -605,53 +676,46 @@ struct Shares {
   __device__ __forceinline__ long long row(int c) const { return c == 0 ? first_row : row0 + c * step; }
 };
 
-// Largest exponent and the sum that goes with it, over all shares; every lane gets both.
-__device__ __forceinline__ void join_stats(const PagedArgs& a, const Shares& s, int lane, float* top, float* sum) {
-  float m = -INFINITY, l = 0.f;
-  for (int c = lane; c < s.n; c += 32) {
-    const float2 st = a.stat[s.row(c)];
-    const float t = fmaxf(m, st.x);
-    l = l * (m == t ? 1.f : exp2f(m - t)) + st.y * (st.x == t ? 1.f : exp2f(st.x - t));
-    m = t;
+// A running sum of shares: m the largest exponent so far, l and o what goes with it.
+struct Joined {
+  float m = -INFINITY, l = 0.f, o = 0.f;
+  __device__ __forceinline__ void add(float2 stat, float part) {
+    const float top = fmaxf(m, stat.x);
+    const float keep = m == top ? 1.f : exp2f(m - top), w = stat.x == top ? 1.f : exp2f(stat.x - top);
+    l = l * keep + w * stat.y;
+    o = o * keep + w * part;
+    m = top;
   }
-  *top = warp_max(m);
-  *sum = warp_sum(l * (m == *top ? 1.f : exp2f(m - *top)));
-}
+};
 
-// Few heads with many shares: a block takes 32 values of one head, its warps every eighth share,
-// whose first loads are under way together with the maxima.
+// Heads with many shares: a block takes 32 values of one head.  All threads look at the exponents, the
+// weights go to shared memory, and each warp takes every eighth share.
 template <class T>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_wide_kernel(const __grid_constant__ PagedArgs a) {
-  constexpr int kAhead = 8;
-  extern __shared__ __align__(16) long long join_prefix[];
-  __shared__ float sums[kJoinWarps][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = a.head_dim, d = blockIdx.y * 32 + lane;
-  const long long share = slab_prefix<kJoinThreads>(a, join_prefix, false);
-  const Shares s(a, join_prefix, share, blockIdx.x / a.heads, blockIdx.x % a.heads);
+  __shared__ float weight[kMostWorkers], smem[32], sums[kJoinWarps][32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, D = a.head_dim, d = blockIdx.y * 32 + lane;
   T* out = static_cast<T*>(a.out) + static_cast<long long>(blockIdx.x) * D;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Shares s(a, blockIdx.x / a.heads, blockIdx.x % a.heads);
   if (s.n < 2) {
     if (s.n == 0 && warp == 0 && d < D) out[d] = from_f<T>(0.f);
     return;
   }
-  float x[kAhead], e[kAhead];
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) {
-    const int c = warp + i * kJoinWarps;
-    x[i] = c < s.n && d < D ? a.part[s.row(c) * D + d] : 0.f;
-    e[i] = c < s.n ? a.stat[s.row(c)].x : -INFINITY;
+  float2 mine = make_float2(-INFINITY, 0.f);
+  for (int c = tid; c < s.n; c += kJoinThreads) {
+    const float2 st = __ldcg(a.stat + s.row(c));
+    const float top = fmaxf(mine.x, st.x);
+    mine.y = mine.y * (mine.x == top ? 1.f : exp2f(mine.x - top)) + st.y * (st.x == top ? 1.f : exp2f(st.x - top));
+    mine.x = top;
+    weight[c] = st.x;
   }
-  float top, sum, o = 0.f;
-  join_stats(a, s, lane, &top, &sum);
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i)
-    if (warp + i * kJoinWarps < s.n) o = fmaf(e[i] == top ? 1.f : exp2f(e[i] - top), x[i], o);
+  const float top = block_max(mine.x, smem);
+  for (int c = tid; c < s.n; c += kJoinThreads) weight[c] = weight[c] == top ? 1.f : exp2f(weight[c] - top);
+  const float sum = block_sum(mine.y * (mine.x == top ? 1.f : exp2f(mine.x - top)), smem);  // synchronises: the weights are there
+  float o = 0.f;
   if (d < D) {
 #pragma unroll 8
-    for (int c = warp + kAhead * kJoinWarps; c < s.n; c += kJoinWarps) {
-      const float ec = a.stat[s.row(c)].x;
-      o = fmaf(ec == top ? 1.f : exp2f(ec - top), a.part[s.row(c) * D + d], o);
-    }
+    for (int c = warp; c < s.n; c += kJoinWarps) o = fmaf(weight[c], __ldcg(a.part + s.row(c) * D + d), o);
   }
   sums[warp][lane] = o;
   __syncthreads();
@@ -662,33 +726,21 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_wide_kernel(const __g
   }
 }
 
-// Many heads with few shares each: one warp per head.
+// Heads with few shares: a warp takes 32 values of one.
 template <class T>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a) {
-  extern __shared__ __align__(16) long long join_prefix[];
-  const int lane = threadIdx.x & 31, D = a.head_dim;
-  const long long share = slab_prefix<kJoinThreads>(a, join_prefix, false);
-  const long long head = static_cast<long long>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
-  if (head >= static_cast<long long>(a.batch) * a.heads) return;
-  const Shares s(a, join_prefix, share, static_cast<int>(head) / a.heads, static_cast<int>(head) % a.heads);
-  T* out = static_cast<T*>(a.out) + head * D;
+  const int lane = threadIdx.x & 31, D = a.head_dim, slices = (D + 31) / 32;
+  const long long task = static_cast<long long>(blockIdx.x) * kJoinWarps + (threadIdx.x >> 5);
+  const int head = static_cast<int>(divide(task, slices)), d = static_cast<int>(task - static_cast<long long>(head) * slices) * 32 + lane;
+  if (head >= a.batch * a.heads) return;
+  T* out = static_cast<T*>(a.out) + static_cast<long long>(head) * D;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (s.n == 1) return;
-  if (s.n == 0) {
-    for (int d = lane; d < D; d += 32) out[d] = from_f<T>(0.f);
-    return;
-  }
-  float top, sum;
-  join_stats(a, s, lane, &top, &sum);
-  for (int d = lane; d < D; d += 32) {
-    float o = 0.f;
+  const Shares s(a, head / a.heads, head % a.heads);
+  if (s.n == 1 || d >= D) return;
+  Joined all;
 #pragma unroll 4
-    for (int c = 0; c < s.n; ++c) {
-      const float e = a.stat[s.row(c)].x;
-      o = fmaf(e == top ? 1.f : exp2f(e - top), a.part[s.row(c) * D + d], o);
-    }
-    out[d] = from_f<T>(o / sum);
-  }
+  for (int c = 0; c < s.n; ++c) all.add(__ldcg(a.stat + s.row(c)), __ldcg(a.part + s.row(c) * D + d));
+  out[d] = from_f<T>(s.n == 0 ? 0.f : all.o / all.l);
 }
 
 // ------------------------------------------------------------------------- host
@@ -724,18 +776,19 @@ void launch_both(Kernel kernel, int threads, size_t smem_ring, PagedArgs a, cons
   blocks = std::min(blocks, kMostWorkers / warps);
   a.workers = blocks * warps;
   const size_t shares = 2ull * a.workers * a.tile_heads;
-  const size_t stat_bytes = (shares * 8 + 255) / 256 * 256;
-  ScratchLease scratch(l.device, stat_bytes + shares * a.head_dim * 4, l.stream);
-  a.stat = static_cast<float2*>(scratch.data());
-  a.part = reinterpret_cast<float*>(static_cast<char*>(scratch.data()) + stat_bytes);
+  const size_t prefix_bytes = (static_cast<size_t>(a.batch) * 8 + 16 + 255) / 256 * 256, stat_bytes = (shares * 8 + 255) / 256 * 256;
+  ScratchLease scratch(l.device, prefix_bytes + stat_bytes + shares * a.head_dim * 4, l.stream);
+  char* at = static_cast<char*>(scratch.data());
+  a.prefix = reinterpret_cast<long long*>(at);
+  a.stat = reinterpret_cast<float2*>(at + prefix_bytes);
+  a.part = reinterpret_cast<float*>(at + prefix_bytes + stat_bytes);
   kernel<<<blocks, threads, smem_ring + (a.batch + 1) * sizeof(long long), l.stream>>>(a, extra...);
   check_launch("paged_attention");
   cudaLaunchConfig_t config{};
   const unsigned heads = static_cast<unsigned>(a.batch) * a.heads, slices = static_cast<unsigned>((a.head_dim + 31) / 32);
-  const bool wide = heads * slices <= 4u * l.sms;
-  config.gridDim = wide ? dim3(heads, slices) : dim3((heads + kJoinWarps - 1) / kJoinWarps);
+  const bool wide = a.workers >= 8ll * a.batch * a.kv_heads * a.tiles;  // shares of a head when all warps have one
+  config.gridDim = wide ? dim3(heads, slices) : dim3(static_cast<unsigned>((static_cast<long long>(heads) * slices + kJoinWarps - 1) / kJoinWarps));
   config.blockDim = dim3(kJoinThreads);
-  config.dynamicSmemBytes = (a.batch + 1) * sizeof(long long);
   config.stream = l.stream;
   cudaLaunchAttribute dependent{};
   dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -21,6 +21,7 @@
 // lanes by their place in the row, exponentials are summed with compensation (to about 2^-45, so
 // that their order hardly matters either), and the sum is rounded to float32 before its logarithm.
 #include <algorithm>
+#include <cmath>
 
 #include "ob/cuda_common.cuh"
 
@@ -28,7 +29,7 @@ namespace ob {
 namespace cu {
 namespace {
 
-constexpr int kWarpsPerSm = 20, kMostLists = 256;  // blocks of one warp; chunks of a sentence that the selection has room for
+constexpr int kWarpsPerSm = 19, kMostLists = 256;  // blocks of one warp; chunks of a sentence that the selection has room for
 constexpr int kBatch = 4, kBatchVectors = kBatch * 32, kRing = 3, kStageBytes = (kBatchVectors + 1) * 16;
 constexpr int kAside = kBatchVectors + 32;  // pieces that a warp has room for: at least a batch at any time
 using Key = unsigned long long;  // order-preserving image of the value, then the complement of its place
@@ -546,15 +547,19 @@ __global__ void __launch_bounds__(32, kWarpsPerSm) beam_step_kernel(const T* __r
     select_beams<T>(logits, a, sentence, *reinterpret_cast<Selection*>(smem));
 }
 
-// Chunks of a beam.  In cycles: an SM that is full takes 82 for a batch (330 instructions of a warp), and a
-// chunk's start and end cost as many instructions as 6; a warp alone needs 900 for a batch.  The sum
-// of the two, everything at full rate and then one chunk to its end, is made small.
+// Chunks of a beam, by an estimate in cycles: a warp alone takes 900 for a batch, n on an SM together 82
+// n; a chunk's start and end take 5500; the selection 3000, and for each of W rounds 600 and a look at
+// all lists.  Chunks that do not fit the device at once cost another round of the same.  (512 rows of
+// 100003: 51 us with 4 or 5 chunks, 57 with 6, 82 with 1; 128 rows of 50021, 16 beams: 37 with 6 to
+// 10, 43 with 16.)
 int choose_chunks(long long rows, int beams, long long vectors, int sms) {
   const double batches = static_cast<double>((vectors + kBatchVectors - 1) / kBatchVectors);
   int best = 1;
   double best_cost = 1e300;
   for (int c = 1; c <= batches && c * beams <= kMostLists; ++c) {
-    const double cost = rows * (batches + 6.0 * c) * 82.0 / sms + (batches / c + 6.0) * 900.0;
+    const double tasks = static_cast<double>(rows) * c, beside = std::min<double>(kWarpsPerSm, std::ceil(tasks / sms));
+    const double rounds = std::ceil(tasks / (kWarpsPerSm * sms));
+    const double cost = rounds * (std::ceil(batches / c) * std::max(900.0, 82.0 * beside) + 5500.0) + 3000.0 + beams * (600.0 + 1.25 * beams * c);
     if (cost < best_cost) { best = c; best_cost = cost; }
   }
   return best;

@@ -13,6 +13,9 @@
 // share in a workspace, and a second kernel joins them in order.  It is launched as a dependent of
 // the first, so that its start-up hides behind it.  No atomics: the same call gives the same bits.
 //
+// Short caches (a table of at most 1024 tokens) are not worth a second kernel: there a block takes one
+// head of one sequence, its warps every slab in turn, and they join in shared memory.
+//
 // Masks.  Rows behind a sequence's length are never read (they are zero-filled on the way in) and
 // weigh nothing; a score of -inf weighs nothing; NaN in what is seen stays NaN.
 #include <algorithm>
@@ -81,6 +84,11 @@ struct Cursor {
     j = static_cast<int>(rest - static_cast<long long>(item) * slabs);
     kv = item / a.tiles;
     tile = item - kv * a.tiles;
+    in_page = j * kSlab % a.page_size;
+  }
+  // The slab `step` behind, of the same head.
+  __device__ __forceinline__ void skip(const PagedArgs& a, int step) {
+    j += step;
     in_page = j * kSlab % a.page_size;
   }
   // Not called behind the last slab of the call.
@@ -177,6 +185,48 @@ __device__ __forceinline__ long long take_share(const PagedArgs& a, long long wo
   return min(share, all * items - lo);
 }
 
+// The block's head, for a block that has one of its own; false where the sequence is empty and the
+// output was set to zero.
+template <class T>
+__device__ __forceinline__ bool take_head(const PagedArgs& a, Cursor* at) {
+  const int row = blockIdx.x / a.tiles, group = a.heads / a.kv_heads;
+  at->tile = blockIdx.x - row * a.tiles;
+  at->b = row / a.kv_heads;
+  at->kv = row - at->b * a.kv_heads;
+  at->n = length_of(a, at->b);
+  at->slabs = slabs_of(at->n);
+  if (at->kv == 0 && at->tile == 0 && threadIdx.x == 0 && at->n != a.lengths[at->b]) atomicAdd(a.errors, 1u);
+  at->j = threadIdx.x >> 5;
+  at->in_page = at->j * kSlab % a.page_size;
+  if (at->n > 0) return true;
+  const int heads = min(a.tile_heads, group - at->tile * a.tile_heads);
+  T* out = static_cast<T*>(a.out) + (static_cast<long long>(at->b) * a.heads + at->kv * group + at->tile * a.tile_heads) * a.head_dim;
+  for (int i = threadIdx.x; i < heads * a.head_dim; i += blockDim.x) out[i] = from_f<T>(0.f);
+  return false;
+}
+
+// The warps' sums of one head tile, in shared memory, into the output.
+template <class T, int WARPS>
+__device__ __forceinline__ void join_warps(const PagedArgs& a, const Cursor& at, int heads, const float2* stat, const float* part) {
+  __syncthreads();
+  const int D = a.head_dim, h0 = at.kv * (a.heads / a.kv_heads) + at.tile * a.tile_heads;
+  T* out = static_cast<T*>(a.out) + (static_cast<long long>(at.b) * a.heads + h0) * D;
+  for (int i = threadIdx.x; i < heads * D; i += WARPS * 32) {
+    const int h = i / D;
+    float top = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, stat[w * heads + h].x);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float2 st = stat[w * heads + h];
+      const float weight = st.x == top ? 1.f : exp2f(st.x - top);
+      sum = fmaf(weight, st.y, sum);
+      o = fmaf(weight, part[(w * heads) * D + i], o);
+    }
+    out[i] = from_f<T>(o / sum);
+  }
+}
+
 // ------------------------------------------------------------- tensor-core warps
 // 16-bit types, head sizes that are a multiple of 8.  With K as the left operand a slab is one
 // m16n8k16 product per 16 values: S^T [16 tokens x 8 heads] = K q^T, and O^T [values x 8 heads]
@@ -231,20 +281,30 @@ struct SlabLayout {
   }
 };
 
-template <class T, int KD, int NT, int STAGES, int WARPS>
+template <class T, int KD, int NT, int STAGES, int WARPS, bool OWN>  // OWN: the block has a head of its own
 __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_constant__ PagedArgs a) {
   using L = SlabLayout<KD>;
   // Weights are at most 2^kLift: float16 then keeps full precision down to 2^-28 of the largest.
   constexpr float kLift = std::is_same<T, __half>::value ? 14.f : 0.f;
   extern __shared__ __align__(1024) unsigned char smem[];
   long long* prefix = reinterpret_cast<long long*>(smem + static_cast<size_t>(WARPS) * STAGES * 2 * L::kBytes);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if constexpr (!OWN) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int D = a.head_dim, group = a.heads / a.kv_heads;
   const long long worker = static_cast<long long>(warp) * gridDim.x + blockIdx.x;  // few slabs spread over all SMs
   Cursor now;
-  const long long mine = take_share<WARPS * 32>(a, worker, prefix, &now);
-  if (mine == 0) return;
+  long long mine;
+  if constexpr (OWN) {
+    if (!take_head<T>(a, &now)) return;
+    mine = now.j < now.slabs ? (now.slabs - now.j + WARPS - 1) / WARPS : 0;
+  } else {
+    mine = take_share<WARPS * 32>(a, worker, prefix, &now);
+    if (mine == 0) return;
+  }
+  auto advance = [&](Cursor& c) {
+    if constexpr (OWN) c.skip(a, WARPS);
+    else c.next(a);
+  };
 
   unsigned char* ring = smem + static_cast<size_t>(warp) * STAGES * 2 * L::kBytes;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
@@ -266,14 +326,15 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
   // load between the copies would wait for them.
   int pages = 0, pages_from = 0, pages_b = -1;
   auto page_of = [&](const Cursor& c) {
-    if (c.b != pages_b || c.j < pages_from || c.j >= pages_from + 32) {
+    constexpr int kStep = OWN ? WARPS : 1;
+    if (c.b != pages_b || c.j < pages_from || c.j >= pages_from + 32 * kStep) {
       pages_b = c.b;
       pages_from = c.j;
-      const int j = c.j + lane;
+      const int j = c.j + lane * kStep;
       pages = j < c.slabs ? a.table[static_cast<long long>(c.b) * a.table_width + j * kSlab / a.page_size] : 0;
       if (j < c.slabs) pages = checked_page(a, pages, true);
     }
-    return __shfl_sync(0xffffffffu, pages, c.j - pages_from);
+    return __shfl_sync(0xffffffffu, pages, (c.j - pages_from) / kStep);
   };
   const long long head_step = static_cast<long long>(a.page_size) * D;
   auto load_slab = [&](int stage, const Cursor& c) {
@@ -340,46 +401,48 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
   for (int s = 0; s < STAGES - 1; ++s) {
     if (to_load > 0) {
       load_slab(s, ahead);
-      if (--to_load > 0) ahead.next(a);
+      if (--to_load > 0) advance(ahead);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
   float o[NT][KD][4], m[NT][2], sum[NT][2];
+  auto clear = [&] {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < KD; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      sum[nt][0] = sum[nt][1] = 0.f;
+    }
+  };
+  clear();
   int stage = 0;
-  bool from_start = false, first_item = true;
+  bool from_start = now.j == 0, first_item = true;
   // ldmatrix addresses: K rows are tokens, (0-7, 8-15) by lane bit 3, pieces by lane bit 4; V transposed, the other way round.
   const int k_row = lane & 15, k_piece = lane >> 4, v_row = (lane & 7) + ((lane >> 4) << 3), v_piece = (lane >> 3) & 1;
 
   for (long long left = mine; left > 0; --left) {
-    if (left == mine || now.j == 0) {  // a new head: its queries, empty sums
-      from_start = now.j == 0;
-      if (left != mine) {
-        if (!kFetchAhead || !fetched || !whose.same_head(now)) load_queries(now, coming);
+    if (!OWN && left != mine && now.j == 0) {  // a new head: its queries, empty sums
+      from_start = true;
+      if (!kFetchAhead || !fetched || !whose.same_head(now)) load_queries(now, coming);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < KD; ++i) {
-            q[nt][i][0] = coming[nt][i][0];
-            q[nt][i][1] = coming[nt][i][1];
-          }
-        fetched = false;
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int i = 0; i < KD; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
-        m[nt][0] = m[nt][1] = -INFINITY;
-        sum[nt][0] = sum[nt][1] = 0.f;
-      }
+        for (int i = 0; i < KD; ++i) {
+          q[nt][i][0] = coming[nt][i][0];
+          q[nt][i][1] = coming[nt][i][1];
+        }
+      fetched = false;
+      clear();
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
     __syncwarp();  // every lane's copies are there, and every lane is done with the slab before
     if (to_load > 0) {
       load_slab(stage == 0 ? STAGES - 1 : stage - 1, ahead);
       if (--to_load > 0) {
-        ahead.next(a);
-        if (kFetchAhead && ahead.j == 0 && !fetched) {  // the next head's queries, while this one's slabs are taken
+        advance(ahead);
+        if (!OWN && kFetchAhead && ahead.j == 0 && !fetched) {  // the next head's queries, while this one's slabs are taken
           load_queries(ahead, coming);
           whose = ahead;
           fetched = true;
@@ -449,7 +512,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
 
-    if (now.j == now.slabs - 1 || left == 1) {  // this share of the head is done
+    if (!OWN && (now.j == now.slabs - 1 || left == 1)) {  // this share of the head is done
       const bool all = from_start && now.j == now.slabs - 1;
       const int h0 = first_head(now), heads = heads_of(now);
       const long long slot = (2 * worker + (first_item ? 0 : 1)) * a.tile_heads;
@@ -482,7 +545,31 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
         }
       first_item = false;
     }
-    if (left > 1) now.next(a);
+    if (left > 1) advance(now);
+  }
+  if constexpr (OWN) {
+    const int heads = heads_of(now);
+    float* part = reinterpret_cast<float*>(smem);
+    float2* stat = reinterpret_cast<float2*>(part + static_cast<size_t>(WARPS) * heads * D);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the rings are done with
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float w = sum[nt][c];
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) w += __shfl_xor_sync(0xffffffffu, w, x);
+        const int h = nt * 8 + t * 2 + c;
+        if (h >= heads) continue;
+        if (g == 0) stat[warp * heads + h] = make_float2(m[nt][c], w);
+#pragma unroll
+        for (int i = 0; i < KD; ++i) {
+          if (i * 16 + g < D) part[(warp * heads + h) * D + i * 16 + g] = o[nt][i][c];
+          if (i * 16 + g + 8 < D) part[(warp * heads + h) * D + i * 16 + g + 8] = o[nt][i][c + 2];
+        }
+      }
+    join_warps<T, WARPS>(a, now, heads, stat, part);
   }
 }
 
@@ -526,25 +613,40 @@ __device__ __forceinline__ float sum_by_halving(float (&x)[N], int lane) {
 }
 
 constexpr int kRowThreads = 256, kRowTokens = 8;
-template <class T, int PER, int NH>
+template <class T, int PER, int NH, bool OWN>
 __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_constant__ PagedArgs a, const bool wide) {
   constexpr int kLaneHeads = NH < 4 ? NH : 4, kSets = NH / kLaneHeads;  // heads that the lanes hold side by side, and how often
   constexpr int kShift = NH == 1 ? 2 : NH == 2 ? 1 : 0;                 // lane = (head, token, copy)
   extern __shared__ __align__(16) long long rows_prefix[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  constexpr int kRowWarps = kRowThreads / 32;
+  if constexpr (!OWN) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d0 = lane * PER;
   const int D = a.head_dim, group = a.heads / a.kv_heads;
   const int my_token = (lane >> kShift) & 7;
   const long long worker = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
   Cursor now;
-  const long long mine = take_share<kRowThreads>(a, worker, rows_prefix, &now);
-  if (mine == 0) return;
+  long long mine;
+  if constexpr (OWN) {
+    if (!take_head<T>(a, &now)) return;
+    mine = now.j < now.slabs ? (now.slabs - now.j + kRowWarps - 1) / kRowWarps : 0;
+  } else {
+    mine = take_share<kRowThreads>(a, worker, rows_prefix, &now);
+    if (mine == 0) return;
+  }
 
   float q[NH][PER], acc[NH][PER], m[kSets], sum[kSets];
   bool from_start = false, first_item = true;
+  if constexpr (OWN) {  // a warp may have no slab at all
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[h][i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < kSets; ++c) { m[c] = -INFINITY; sum[c] = 0.f; }
+  }
   for (long long left = mine; left > 0; --left) {
     const int h0 = now.kv * group + now.tile * a.tile_heads, heads = min(a.tile_heads, group - now.tile * a.tile_heads);
-    if (left == mine || now.j == 0) {
+    if (left == mine || (!OWN && now.j == 0)) {
       from_start = now.j == 0;
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
@@ -622,7 +724,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
           for (int i = 0; i < PER; ++i) acc[h][i] = fmaf(w, to_f(v[u].v[i]), acc[h][i]);
         }
     }
-    if (now.j == now.slabs - 1 || left == 1) {
+    if (!OWN && (now.j == now.slabs - 1 || left == 1)) {
       const bool all = from_start && now.j == now.slabs - 1;
       const long long slot = (2 * worker + (first_item ? 0 : 1)) * a.tile_heads;
 #pragma unroll
@@ -646,7 +748,28 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const __grid_co
       }
       first_item = false;
     }
-    if (left > 1) now.next(a);
+    if constexpr (OWN) now.skip(a, kRowWarps);
+    else if (left > 1) now.next(a);
+  }
+  if constexpr (OWN) {
+    const int heads = min(a.tile_heads, group - now.tile * a.tile_heads);
+    float* part = reinterpret_cast<float*>(rows_prefix);
+    float2* stat = reinterpret_cast<float2*>(part + static_cast<size_t>(kRowWarps) * NH * D);
+#pragma unroll
+    for (int c = 0; c < kSets; ++c)
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) sum[c] += __shfl_xor_sync(0xffffffffu, sum[c], o << kShift);
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      const float w = __shfl_sync(0xffffffffu, sum[h / kLaneHeads], (h % kLaneHeads) << (kShift + 3));
+      const float top = __shfl_sync(0xffffffffu, m[h / kLaneHeads], (h % kLaneHeads) << (kShift + 3));
+      if (h >= heads) continue;
+      if (lane == 0) stat[warp * heads + h] = make_float2(top, w);
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (d0 + i < D) part[(warp * heads + h) * D + d0 + i] = acc[h][i];
+    }
+    join_warps<T, kRowWarps>(a, now, heads, stat, part);
   }
 }
 
@@ -799,15 +922,32 @@ void launch_both(Kernel kernel, int threads, size_t smem_ring, PagedArgs a, cons
   check_launch("paged_attention join");
 }
 
-template <class T, int KD, int STAGES, int WARPS>
+// One block for each head tile of each sequence.
+template <class Kernel, class... Extra>
+void launch_own(Kernel kernel, int threads, size_t smem, const PagedArgs& a, const Launch& l, Extra... extra) {
+  blocks_per_sm(kernel, l.device.index, threads, smem);
+  kernel<<<static_cast<unsigned>(a.batch) * a.kv_heads * a.tiles, threads, smem, l.stream>>>(a, extra...);
+  check_launch("paged_attention");
+}
+
+// With a block per head: 333 tokens, 16 heads of 128: 7 us instead of 12; 64 sequences of up to 512, 8 heads of 64: see below.
+bool short_cache(const PagedArgs& a) { return static_cast<long long>(a.table_width) * a.page_size <= 1024; }
+
+template <class T, int KD, int NT, int STAGES, int WARPS, int OWN_STAGES>
 void launch_tiles(PagedArgs a, const Launch& l) {
-  const int group = a.heads / a.kv_heads;
-  const int most = group <= 8 ? 8 : 16;
+  const int group = a.heads / a.kv_heads, most = 8 * NT;
   a.tiles = (group + most - 1) / most;
   a.tile_heads = (group + a.tiles - 1) / a.tiles;
-  const size_t ring = static_cast<size_t>(WARPS) * STAGES * 2 * SlabLayout<KD>::kBytes;
-  if (most == 8) launch_both<T>(paged_tile_kernel<T, KD, 1, STAGES, WARPS>, WARPS * 32, ring, a, l);
-  else launch_both<T>(paged_tile_kernel<T, KD, 2, STAGES, WARPS>, WARPS * 32, ring, a, l);
+  constexpr size_t slab = 2 * SlabLayout<KD>::kBytes;
+  if (short_cache(a)) launch_own(paged_tile_kernel<T, KD, NT, OWN_STAGES, 4, true>, 128, 4 * OWN_STAGES * slab, a, l);
+  else launch_both<T>(paged_tile_kernel<T, KD, NT, STAGES, WARPS, false>, WARPS * 32, WARPS * STAGES * slab, a, l);
+}
+
+template <class T, int PER, int NH>
+void launch_rows(const PagedArgs& a, const Launch& l, bool wide) {
+  const size_t own = kRowThreads / 32 * static_cast<size_t>(NH) * (a.head_dim * sizeof(float) + sizeof(float2));
+  if (short_cache(a)) launch_own(paged_rows_kernel<T, PER, NH, true>, kRowThreads, own, a, l, wide);
+  else launch_both<T>(paged_rows_kernel<T, PER, NH, false>, kRowThreads, 0, a, l, wide);
 }
 
 template <class T, int PER>
@@ -816,10 +956,10 @@ void launch_rows(PagedArgs a, const Launch& l, bool wide) {
   const int most = PER == 8 ? 4 : 8;  // registers: queries and sums are NH x PER values each
   a.tiles = (group + most - 1) / most;
   a.tile_heads = (group + a.tiles - 1) / a.tiles;
-  if (a.tile_heads == 1) launch_both<T>(paged_rows_kernel<T, PER, 1>, kRowThreads, 0, a, l, wide);
-  else if (a.tile_heads == 2) launch_both<T>(paged_rows_kernel<T, PER, 2>, kRowThreads, 0, a, l, wide);
-  else if (a.tile_heads <= 4) launch_both<T>(paged_rows_kernel<T, PER, 4>, kRowThreads, 0, a, l, wide);
-  else if constexpr (PER < 8) launch_both<T>(paged_rows_kernel<T, PER, 8>, kRowThreads, 0, a, l, wide);
+  if (a.tile_heads == 1) launch_rows<T, PER, 1>(a, l, wide);
+  else if (a.tile_heads == 2) launch_rows<T, PER, 2>(a, l, wide);
+  else if (a.tile_heads <= 4) launch_rows<T, PER, 4>(a, l, wide);
+  else if constexpr (PER < 8) launch_rows<T, PER, 8>(a, l, wide);
 }
 
 template <class T>
@@ -828,10 +968,12 @@ void attend(const PagedArgs& a, const Launch& l) {
   const uintptr_t bases = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
   if constexpr (sizeof(T) == 2) {
     if (a.head_dim % 8 == 0 && strides % 8 == 0 && bases % 16 == 0) {
-      if (a.head_dim <= 64) launch_tiles<T, 4, 6, 8>(a, l);
-      else if (a.head_dim <= 96) launch_tiles<T, 6, 4, 8>(a, l);
-      else if (a.head_dim <= 128) launch_tiles<T, 8, 3, 8>(a, l);
-      else launch_tiles<T, 16, 3, 4>(a, l);
+      // Up to 8 query heads of a cached head fill one product; more warps where a slab is short.
+      const bool one = a.heads / a.kv_heads <= 8;
+      if (a.head_dim <= 64) one ? launch_tiles<T, 4, 1, 3, 16, 4>(a, l) : launch_tiles<T, 4, 2, 6, 8, 4>(a, l);
+      else if (a.head_dim <= 96) one ? launch_tiles<T, 6, 1, 2, 12, 3>(a, l) : launch_tiles<T, 6, 2, 4, 8, 3>(a, l);
+      else if (a.head_dim <= 128) one ? launch_tiles<T, 8, 1, 3, 8, 3>(a, l) : launch_tiles<T, 8, 2, 3, 8, 3>(a, l);
+      else one ? launch_tiles<T, 16, 1, 3, 4, 3>(a, l) : launch_tiles<T, 16, 2, 3, 4, 3>(a, l);
       return;
     }
   }

@@ -13,8 +13,8 @@
 // share in a workspace, and a second kernel joins them in order.  It is launched as a dependent of
 // the first, so that its start-up hides behind it.  No atomics: the same call gives the same bits.
 //
-// Short caches (a table of at most 1024 tokens) are not worth a second kernel: there a block takes one
-// head of one sequence, its warps every slab in turn, and they join in shared memory.
+// Short caches are not worth a second kernel, and many heads need no division: there a block takes
+// one head of one sequence, its warps every slab in turn, and they join in shared memory.
 //
 // Masks.  Rows behind a sequence's length are never read (they are zero-filled on the way in) and
 // weigh nothing; a score of -inf weighs nothing; NaN in what is seen stays NaN.
@@ -930,8 +930,16 @@ void launch_own(Kernel kernel, int threads, size_t smem, const PagedArgs& a, con
   check_launch("paged_attention");
 }
 
-// With a block per head: 333 tokens, 16 heads of 128: 7 us instead of 12; 64 sequences of up to 512, 8 heads of 64: see below.
-bool short_cache(const PagedArgs& a) { return static_cast<long long>(a.table_width) * a.page_size <= 1024; }
+// A block per head, or even shares and a second kernel?  The second kernel costs about 7 us; a block alone
+// takes 0.0094 us for a token of 512 bytes, until 1.6 heads on each SM keep the memory busy.  Lengths
+// are on the device: what the table has room for stands for them, and a table beyond 4096 tokens,
+// where one long sequence could keep a few blocks running alone, gets even shares.  (Own against
+// shares, 8 cached heads of 128: 1 sequence of 512 tokens 10.3 / 13.7 us, 1024 14.5 / 14.3, 2048 24.7 /
+// 16.4; 16 of up to 2048 26.5 / 32.8; 64 of up to 2048 58.7 / 67.5; 8 of 8192 84.4 / 58.4.)
+bool block_per_head(const PagedArgs& a, int sms) {
+  const double room = static_cast<double>(a.table_width) * a.page_size, heads = static_cast<double>(a.batch) * a.kv_heads * a.tiles;
+  return room <= 4096.0 && (1.0 - heads / (1.6 * sms)) * room <= 1000.0;
+}
 
 template <class T, int KD, int NT, int STAGES, int WARPS, int OWN_STAGES>
 void launch_tiles(PagedArgs a, const Launch& l) {
@@ -939,14 +947,14 @@ void launch_tiles(PagedArgs a, const Launch& l) {
   a.tiles = (group + most - 1) / most;
   a.tile_heads = (group + a.tiles - 1) / a.tiles;
   constexpr size_t slab = 2 * SlabLayout<KD>::kBytes;
-  if (short_cache(a)) launch_own(paged_tile_kernel<T, KD, NT, OWN_STAGES, 4, true>, 128, 4 * OWN_STAGES * slab, a, l);
+  if (block_per_head(a, l.sms)) launch_own(paged_tile_kernel<T, KD, NT, OWN_STAGES, 4, true>, 128, 4 * OWN_STAGES * slab, a, l);
   else launch_both<T>(paged_tile_kernel<T, KD, NT, STAGES, WARPS, false>, WARPS * 32, WARPS * STAGES * slab, a, l);
 }
 
 template <class T, int PER, int NH>
 void launch_rows(const PagedArgs& a, const Launch& l, bool wide) {
   const size_t own = kRowThreads / 32 * static_cast<size_t>(NH) * (a.head_dim * sizeof(float) + sizeof(float2));
-  if (short_cache(a)) launch_own(paged_rows_kernel<T, PER, NH, true>, kRowThreads, own, a, l, wide);
+  if (block_per_head(a, l.sms)) launch_own(paged_rows_kernel<T, PER, NH, true>, kRowThreads, own, a, l, wide);
   else launch_both<T>(paged_rows_kernel<T, PER, NH, false>, kRowThreads, 0, a, l, wide);
 }
 
@@ -968,7 +976,8 @@ void attend(const PagedArgs& a, const Launch& l) {
   const uintptr_t bases = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
   if constexpr (sizeof(T) == 2) {
     if (a.head_dim % 8 == 0 && strides % 8 == 0 && bases % 16 == 0) {
-      // Up to 8 query heads of a cached head fill one product; more warps where a slab is short.
+      // Up to 8 query heads of a cached head fill one product; more warps where a slab is short: it takes
+      // a warp about as long whatever its bytes (128 sequences of up to 2000, 16 heads of 64: 16 warps 96 us).
       const bool one = a.heads / a.kv_heads <= 8;
       if (a.head_dim <= 64) one ? launch_tiles<T, 4, 1, 3, 16, 4>(a, l) : launch_tiles<T, 4, 2, 6, 8, 4>(a, l);
       else if (a.head_dim <= 96) one ? launch_tiles<T, 6, 1, 2, 12, 3>(a, l) : launch_tiles<T, 6, 2, 4, 8, 3>(a, l);

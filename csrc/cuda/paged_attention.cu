@@ -10,8 +10,9 @@
 // the order (sequence, head, token), are divided evenly over the warps of a persistent grid, whatever
 // the lengths are: a warp streams its own slabs and meets no other on the way.  A head that lies
 // within one warp's share is written at once; one that is spread leaves (m, sum p, sum p v) of each
-// share in a workspace, and a second kernel joins them in order.  It is launched as a dependent of
-// the first, so that its start-up hides behind it.  No atomics: the same call gives the same bits.
+// share in a workspace, and a second kernel joins them in order.  No atomics: the same call gives the
+// same bits.  (Joining inside the first kernel, by the last warp to arrive, was measured too: 116 us
+// instead of 99 for 131072 tokens, because its fences wait for the streams around it.)
 //
 // Short caches are not worth a second kernel, and many heads need no division: there a block takes
 // one head of one sequence, its warps every slab in turn, and they join in shared memory.
@@ -74,7 +75,7 @@ __device__ __forceinline__ int slabs_of(int n) { return (n + kSlab - 1) / kSlab;
 struct Cursor {
   int b, kv, tile;   // sequence, cached head, tile of its query heads
   int j, slabs, n;   // slab of it; slabs of it; length of the sequence
-  int in_page;       // first token's place in its page, where pages are a multiple of slabs
+  int in_page;       // first token's place in its page
   // `rest`: slabs behind the first of sequence `at`.
   __device__ __forceinline__ void set(const PagedArgs& a, int at, int length, long long rest) {
     b = at;
@@ -94,7 +95,7 @@ struct Cursor {
   // Not called behind the last slab of the call.
   __device__ __forceinline__ void next(const PagedArgs& a) {
     in_page += kSlab;
-    if (in_page >= a.page_size) in_page = 0;
+    while (in_page >= a.page_size) in_page -= a.page_size;
     if (++j < slabs) return;
     j = in_page = 0;
     if (++tile < a.tiles) return;
@@ -108,6 +109,14 @@ struct Cursor {
   }
   __device__ __forceinline__ bool same_head(const Cursor& c) const { return b == c.b && kv == c.kv && tile == c.tile; }
 };
+
+// Slabs of one share: all warps get one, but few shares of a long head are cheaper to join.  A slab
+// takes a warp 750 cycles and 64 shares take the joining block 900, so a head of n slabs wants shares
+// of sqrt(n / 50) at least (2 heads of 15954 tokens: 28.5 us with shares of 2).
+__device__ __forceinline__ long long share_of(const PagedArgs& a, long long all) {
+  const long long even = divide(all * a.kv_heads * a.tiles + a.workers - 1, a.workers);
+  return max(even, static_cast<long long>(ceilf(sqrtf(0.02f * static_cast<float>(all) / static_cast<float>(a.batch)))));
+}
 
 // The share of this warp: warp c of the grid takes the slabs from c * share on.  Returns how many,
 // and the first of them in `at`.  Block 0 leaves the slabs before each sequence and the share for the
@@ -128,7 +137,7 @@ __device__ __forceinline__ long long take_share(const PagedArgs& a, long long wo
       if (lane >= o) run += x;
     }
     all = __shfl_sync(0xffffffffu, run, a.batch - 1);
-    const long long share = divide(all * items + a.workers - 1, a.workers), lo = worker * share;
+    const long long share = share_of(a, all), lo = worker * share;
     if (tell && threadIdx.x < a.batch) a.prefix[lane] = run - mine;
     if (tell && threadIdx.x == 0) {
       a.prefix[a.batch] = all;
@@ -168,7 +177,7 @@ __device__ __forceinline__ long long take_share(const PagedArgs& a, long long wo
     before += slabs_of(length_of(a, b));
   }
   __syncthreads();
-  const long long share = divide(all * items + a.workers - 1, a.workers), lo = worker * share;
+  const long long share = share_of(a, all), lo = worker * share;
   if (tell && threadIdx.x == 0) {
     a.prefix[a.batch] = all;
     a.prefix[a.batch + 1] = share;
@@ -316,50 +325,57 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
     }
     __syncwarp();
   }
-  const bool whole_pages = a.page_size % kSlab == 0;  // then a slab lies within one page, its rows together
+  // Pages of a multiple of 16 tokens hold a slab each, its rows together; of 8, half a slab.
+  const bool whole_pages = a.page_size % kSlab == 0, half_pages = !whole_pages && a.page_size % 8 == 0;
   const int magic = (65536 + real - 1) / real;        // c / real for c < 512
 
   Cursor ahead = now;
   long long to_load = mine;
 
-  // Page numbers of the next slabs of one head, one in each lane: fetched 32 at a time, because a
-  // load between the copies would wait for them.
+  // Page numbers of the next slabs (half slabs) of one head, one in each lane: fetched 32 at a time,
+  // because a load between the copies would wait for them.
   int pages = 0, pages_from = 0, pages_b = -1;
-  auto page_of = [&](const Cursor& c) {
+  auto page_of = [&](const Cursor& c, int half) {
     constexpr int kStep = OWN ? WARPS : 1;
-    if (c.b != pages_b || c.j < pages_from || c.j >= pages_from + 32 * kStep) {
+    const int log_halves = half_pages ? 1 : 0;
+    if (c.b != pages_b || c.j < pages_from || c.j >= pages_from + (32 >> log_halves) * kStep) {
       pages_b = c.b;
       pages_from = c.j;
-      const int j = c.j + lane * kStep;
-      pages = j < c.slabs ? a.table[static_cast<long long>(c.b) * a.table_width + j * kSlab / a.page_size] : 0;
-      if (j < c.slabs) pages = checked_page(a, pages, true);
+      const int j = c.j + (lane >> log_halves) * kStep, token = j * kSlab + (lane & log_halves) * 8;
+      pages = token < c.n ? a.table[static_cast<long long>(c.b) * a.table_width + token / a.page_size] : 0;
+      if (token < c.n) pages = checked_page(a, pages, true);
     }
-    return __shfl_sync(0xffffffffu, pages, (c.j - pages_from) / kStep);
+    return __shfl_sync(0xffffffffu, pages, ((c.j - pages_from) / kStep << log_halves) + half);
   };
   const long long head_step = static_cast<long long>(a.page_size) * D;
   auto load_slab = [&](int stage, const Cursor& c) {
     const int n = c.n - c.j * kSlab;  // rows of the slab that exist
     const uint32_t to = ring_at + stage * 2 * L::kBytes;
-    if (whole_pages) {
-      const int page = page_of(c);
-      const long long inner = c.kv * head_step + (c.in_page * D + lane * 8);
-      const T* k = static_cast<const T*>(a.k) + (page * a.page_stride[0] + inner);
-      const T* v = static_cast<const T*>(a.v) + (page * a.page_stride[1] + inner);
+    if (whole_pages || half_pages) {
+      // Row r of the slab at k[half] + r * D, half = r / 8.
+      const T *k[2], *v[2];
+      const int page = page_of(c, 0), last = half_pages ? page_of(c, 1) : page;
+      const int next = half_pages && c.in_page + 8 == a.page_size ? -8 : c.in_page;  // of the second half, less 8
+      const long long inner = c.kv * head_step + lane * 8;
+      k[0] = static_cast<const T*>(a.k) + (page * a.page_stride[0] + inner + c.in_page * D);
+      v[0] = static_cast<const T*>(a.v) + (page * a.page_stride[1] + inner + c.in_page * D);
+      k[1] = static_cast<const T*>(a.k) + (last * a.page_stride[0] + inner + next * D);
+      v[1] = static_cast<const T*>(a.v) + (last * a.page_stride[1] + inner + next * D);
       if (real == L::kChunks && n >= kSlab) {
 #pragma unroll
         for (int i = 0; i < L::kChunks / 2; ++i) {
-          const int x = i * 32 + lane;
+          const int x = i * 32 + lane, half = i * 32 / L::kChunks / 8;
           const uint32_t at = to + L::at(x / L::kChunks, x % L::kChunks);
-          copy16(at, k + i * 256);
-          copy16(at + L::kBytes, v + i * 256);
+          copy16(at, k[half] + i * 256);
+          copy16(at + L::kBytes, v[half] + i * 256);
         }
       } else {
 #pragma unroll 1
-        for (int x = lane; x < kSlab * real; x += 32, k += 256, v += 256) {
+        for (int x = lane, i = 0; x < kSlab * real; x += 32, i += 256) {
           const int row = (x * magic) >> 16;
           const uint32_t at = to + L::at(row, x - row * real);
-          copy16_or_zero(at, k, row < n);
-          copy16_or_zero(at + L::kBytes, v, row < n);
+          copy16_or_zero(at, (row < 8 ? k[0] : k[1]) + i, row < n);
+          copy16_or_zero(at + L::kBytes, (row < 8 ? v[0] : v[1]) + i, row < n);
         }
       }
     } else {
@@ -917,7 +933,7 @@ void launch_both(Kernel kernel, int threads, size_t smem_ring, PagedArgs a, cons
   dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   dependent.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &dependent;
-  config.numAttrs = 1;
+  config.numAttrs = wide ? 0 : 1;  // few blocks that wait on the first kernel's SMs only slow it (131072 tokens: 99 us, 96 without)
   OB_CUDA(cudaLaunchKernelEx(&config, wide ? paged_join_wide_kernel<T> : paged_join_kernel<T>, static_cast<const PagedArgs&>(a)));
   check_launch("paged_attention join");
 }

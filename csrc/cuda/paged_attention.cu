@@ -341,9 +341,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
     if (c.b != pages_b || c.j < pages_from || c.j >= pages_from + (32 >> log_halves) * kStep) {
       pages_b = c.b;
       pages_from = c.j;
-      const int j = c.j + (lane >> log_halves) * kStep, token = j * kSlab + (lane & log_halves) * 8;
-      pages = token < c.n ? a.table[static_cast<long long>(c.b) * a.table_width + token / a.page_size] : 0;
-      if (token < c.n) pages = checked_page(a, pages, true);
+      const unsigned j = c.j + (lane >> log_halves) * kStep, token = j * kSlab + (lane & log_halves) * 8;  // may pass 2^31
+      const bool there = token < static_cast<unsigned>(c.n);
+      pages = there ? a.table[static_cast<long long>(c.b) * a.table_width + token / static_cast<unsigned>(a.page_size)] : 0;
+      if (there) pages = checked_page(a, pages, true);
     }
     return __shfl_sync(0xffffffffu, pages, ((c.j - pages_from) / kStep << log_halves) + half);
   };
@@ -355,10 +356,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
       // Row r of the slab at k[half] + r * D, half = r / 8.
       const T *k[2], *v[2];
       const int page = page_of(c, 0), last = half_pages ? page_of(c, 1) : page;
-      const int next = half_pages && c.in_page + 8 == a.page_size ? -8 : c.in_page;  // of the second half, less 8
+      const long long in_page = c.in_page, next = half_pages && c.in_page + 8 == a.page_size ? -8 : c.in_page;  // of the second half, less 8
       const long long inner = c.kv * head_step + lane * 8;
-      k[0] = static_cast<const T*>(a.k) + (page * a.page_stride[0] + inner + c.in_page * D);
-      v[0] = static_cast<const T*>(a.v) + (page * a.page_stride[1] + inner + c.in_page * D);
+      k[0] = static_cast<const T*>(a.k) + (page * a.page_stride[0] + inner + in_page * D);
+      v[0] = static_cast<const T*>(a.v) + (page * a.page_stride[1] + inner + in_page * D);
       k[1] = static_cast<const T*>(a.k) + (last * a.page_stride[0] + inner + next * D);
       v[1] = static_cast<const T*>(a.v) + (last * a.page_stride[1] + inner + next * D);
       if (real == L::kChunks && n >= kSlab) {
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
         const int slot = token / a.page_size;
         const int entry = row < n ? a.table[static_cast<long long>(c.b) * a.table_width + slot] : 0;
         const int pg = checked_page(a, entry, chunk == 0);
-        const long long inner = c.kv * head_step + (token - slot * a.page_size) * D + chunk * 8;
+        const long long inner = c.kv * head_step + static_cast<long long>(token - slot * a.page_size) * D + chunk * 8;
         const uint32_t at = to + L::at(row, chunk);
         copy16_or_zero(at, static_cast<const T*>(a.k) + (row < n ? pg * a.page_stride[0] + inner : 0), row < n);
         copy16_or_zero(at + L::kBytes, static_cast<const T*>(a.v) + (row < n ? pg * a.page_stride[1] + inner : 0), row < n);
@@ -941,7 +942,7 @@ void launch_both(Kernel kernel, int threads, size_t smem_ring, PagedArgs a, cons
 // One block for each head tile of each sequence.
 template <class Kernel, class... Extra>
 void launch_own(Kernel kernel, int threads, size_t smem, const PagedArgs& a, const Launch& l, Extra... extra) {
-  blocks_per_sm(kernel, l.device.index, threads, smem);
+  blocks_per_sm(kernel, l.device.index, threads, smem);  // opts in to `smem`, the same in every call
   kernel<<<static_cast<unsigned>(a.batch) * a.kv_heads * a.tiles, threads, smem, l.stream>>>(a, extra...);
   check_launch("paged_attention");
 }
@@ -969,7 +970,7 @@ void launch_tiles(PagedArgs a, const Launch& l) {
 
 template <class T, int PER, int NH>
 void launch_rows(const PagedArgs& a, const Launch& l, bool wide) {
-  const size_t own = kRowThreads / 32 * static_cast<size_t>(NH) * (a.head_dim * sizeof(float) + sizeof(float2));
+  constexpr size_t own = kRowThreads / 32 * static_cast<size_t>(NH) * (PER * 32 * sizeof(float) + sizeof(float2));  // for every head size of the kernel
   if (block_per_head(a, l.sms)) launch_own(paged_rows_kernel<T, PER, NH, true>, kRowThreads, own, a, l, wide);
   else launch_both<T>(paged_rows_kernel<T, PER, NH, false>, kRowThreads, 0, a, l, wide);
 }

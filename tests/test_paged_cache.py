@@ -103,6 +103,59 @@ def test_attention_matches_the_definition(device, dtype, lengths, H, K, D, P):
 
 
 @pytest.mark.parametrize("device,dtype", DEVICES)
+@pytest.mark.parametrize("room", [0, 5000])
+@pytest.mark.parametrize("lengths,H,K,D,P", CASES[:5] + [
+    ([100, 7, 24, 0, 49], 8, 1, 128, 8), ([30, 70, 1, 25], 4, 2, 64, 24), ([90, 8], 20, 1, 80, 8), ([60, 0, 16], 10, 1, 256, 16), ([31] * 3, 40, 1, 96, 40),
+    ([77, 3], 40, 2, 64, 16), ([50, 1, 200], 5, 1, 96, 32), ([9, 70], 12, 4, 20, 4), ([40, 13], 6, 1, 33, 5), ([1000, 1, 0, 513], 2, 2, 256, 64),
+    ([700, 0, 3] * 12, 4, 2, 128, 16), ([17, 0, 40, 1, 5, 16, 33] * 300, 2, 1, 64, 16)])
+def test_tables_with_room_for_more(device, dtype, room, lengths, H, K, D, P):
+    """The result does not depend on the table's width, by which the kernel chooses how it divides the work."""
+    rng = np.random.default_rng(len(lengths) + H + D + 1)
+    table, pages = make_table(rng, lengths, P)
+    table = np.pad(table, ((0, 0), (0, max(0, -(-room // P) - table.shape[1]))), constant_values=pages - 1)
+    q = give(rng.standard_normal((len(lengths), H, D)) * 2, dtype, device)
+    kp, vp = (give(x, dtype, device) for x in rng.standard_normal((2, pages, K, P, D)))
+    got = ob.paged_attention(q, kp, vp, whole(table, device), whole(lengths, device))
+    check_attention(got, seen(q), seen(kp), seen(vp), table, lengths, D ** -0.5, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spare", [16, 24, 17])
+def test_pages_beyond_32_bits(spare):
+    """Pages of more than 2^31 values: zeros but for the last three tokens."""
+    N, D, dev = 2 ** 24 + spare, 128, "cuda:0"
+    rng = np.random.default_rng(spare)
+    kp, vp = (_C._zeros_on([2, 1, N, D], "bfloat16", dev) for _ in range(2))
+    k, v, q = (give(rng.standard_normal(s), "bfloat16", dev) for s in ((1, 3, 1, D), (1, 3, 1, D), (1, 2, D)))
+    table, n = whole([[1]], dev), whole([N], dev)
+    ob.paged_append_(kp, vp, k, v, table, whole([N - 3], dev))
+    got = seen(ob.paged_attention(q, kp, vp, table, n, scale=1.0))
+    s = np.einsum("hd,td->ht", seen(q)[0], seen(k)[0, :, 0])
+    top = np.maximum(s.max(-1, keepdims=True), 0.0)
+    p = np.exp(s - top)
+    total = p.sum(-1, keepdims=True) + (N - 3) * np.exp(-top)
+    want = p / total @ seen(v)[0, :, 0]
+    # Half a step for a weight, half a step for the result, and the sums of N zeros' equal weights: at most N 2^-24 = 1 step
+    # of float32 for each of the few thousand that a warp adds, which the half steps of bfloat16 leave room for.
+    size = p / total @ abs(seen(v)[0, :, 0])
+    assert (abs(got[0] - want) <= 2.0 ** -8 * abs(want) + (2.0 ** -8 + 2 ** -9) * size).all()
+    ob.copy_pages_(kp, [1], [0])
+    assert np.array_equal(seen(kp.slice(0, 0, 1).slice(2, N - 3, N))[0, 0], seen(k)[0, :, 0])
+
+
+@pytest.mark.parametrize("device,dtype", DEVICES)
+def test_head_sizes_one_after_another(device, dtype):
+    """Small heads first: what a launch asks the device for does not depend on what was asked before."""
+    rng = np.random.default_rng(6)
+    for D in (24, 33, 60, 64, 65, 120, 128, 130, 256):
+        for H in (1, 2, 3, 8):
+            table, pages = make_table(rng, [20, 3], 16)
+            q, kp, vp = (give(rng.standard_normal(s), dtype, device) for s in ((2, H, D), (pages, 1, 16, D), (pages, 1, 16, D)))
+            got = ob.paged_attention(q, kp, vp, whole(table, device), whole([20, 3], device))
+            check_attention(got, seen(q), seen(kp), seen(vp), table, [20, 3], D ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("device,dtype", DEVICES)
 @pytest.mark.parametrize("D,P,H", [(64, 16, 4), (128, 32, 2), (40, 8, 2)])
 def test_what_lies_behind_the_length_does_not_matter(device, dtype, D, P, H):
     """NaN and infinities in the unused rows of the last page, in pages that belong to nobody, and in wrong table entries

@@ -143,6 +143,11 @@ void paged_attention_cpu(OpCall& c) {
   });
 }
 
+// Beams that offer the same scores tie, whatever order their exponentials were summed in: the
+// logarithm of the sum is rounded to 2^-30, far above the noise of the summation (about 2^-45) and
+// far below what scores are known to (2^-24 of their size).
+double round_log_sum(double log_sum) { return std::nearbyint(log_sum * 1073741824.0) * (1.0 / 1073741824.0); }
+
 template <class T>
 void beam_step_cpu(OpCall& c) {
   const Tensor &logits = c.in[0], &scores = c.in[1], &finished = c.in[2];

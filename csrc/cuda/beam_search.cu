@@ -2,7 +2,10 @@
 //
 //   candidate (w, v) = score_w + x_wv - lse_w,   lse_w = log sum_v exp x_wv
 //
-// The logits are read once; that is the floor.  Within a beam the order of the candidates is the
+// The logits are read once; that is the floor (512 rows of 100003 in bfloat16, every fifth at its end:
+// 82 MB, 12.5 us).  It takes 46 us: a batch of 1024 logits costs a warp about 330 instructions, of
+// which exponentials and their compensated sum are half, and 11 warps on an SM get through one in
+// 150 cycles; the start of a warp, with cold code, and the selection are 10 us.  Within a beam the order of the candidates is the
 // order of the logits, so the beams are cut into chunks, and a warp takes from one its W best (value,
 // lowest place) together with its maximum and sum of exponentials, in one pass.  The last warp of a
 // sentence to arrive forms each beam's lse and picks the W best of the chunks' winners, in float64.
@@ -432,7 +435,8 @@ __device__ __noinline__ void fill_up(const T* logits, const Selection* sh, float
 
 // The selection of one sentence from its chunks' winners; by one warp.  The chunks' lists are in
 // order: W times the best of their heads is taken, and its list moves on.  The warp comes here once
-// and finds the code in no instruction cache, so it is short loops rather than fast ones.
+// and finds the code in no instruction cache, so it is short loops rather than fast ones.  A round
+// takes 850 cycles (1200 with shuffles of all 128 bits in place of the reductions).
 template <class T>
 __device__ __forceinline__ void select_beams(const T* __restrict__ logits, const BeamArgs& a, int sentence, Selection& sh) {
   const int W = a.beams, C = a.chunks, lane = threadIdx.x, lists = W * C;
@@ -498,36 +502,60 @@ __device__ __forceinline__ void select_beams(const T* __restrict__ logits, const
   __syncwarp();
   Key coming = 0;  // a list's entry on its way from memory; it is needed a round later at the earliest
   int comes_to = -1, n = 0;
-#pragma unroll 1
-  for (; n < W; ++n) {
-    Key best = 0, place = ~0ull;
-    int from = -1;
+  Key best, place;  // of the lane's own lists
+  int from = 0;
+  auto look = [&] {
+    best = 0;
+    place = ~0ull;
 #pragma unroll 1
     for (int i = lane; i < lists; i += 32) {
       const Key o = sh.list[i].order, p = sh.list[i].place;
       if (o > best || (o == best && o != 0 && p < place)) { best = o; place = p; from = i; }
     }
-    Key top = best, top_place = place;
+  };
+  look();
+  Key chosen[2], chosen_place[2];  // entry n is lane n % 32's; all are written together
 #pragma unroll 1
-    for (int x = 16; x > 0; x >>= 1) {
-      const Key o = __shfl_xor_sync(0xffffffffu, top, x), p = __shfl_xor_sync(0xffffffffu, top_place, x);
-      if (o > top || (o == top && p < top_place)) { top = o; top_place = p; }
+  for (; n < W; ++n) {
+    const unsigned upper = static_cast<unsigned>(best >> 32), top_upper = __reduce_max_sync(0xffffffffu, upper);
+    const unsigned lower = static_cast<unsigned>(best), top_lower = __reduce_max_sync(0xffffffffu, upper == top_upper ? lower : 0u);
+    if ((top_upper | top_lower) == 0) break;
+    bool holds = upper == top_upper && lower == top_lower;
+    unsigned who = __ballot_sync(0xffffffffu, holds);
+    if ((who & (who - 1)) != 0) {  // equal scores: the lowest beam, then the lowest token
+      const unsigned w = static_cast<unsigned>(place >> 32), v = static_cast<unsigned>(place);
+      const unsigned least_w = __reduce_min_sync(0xffffffffu, holds ? w : ~0u);  // by all lanes, whatever they hold
+      holds = holds && w == least_w;
+      const unsigned least_v = __reduce_min_sync(0xffffffffu, holds ? v : ~0u);
+      holds = holds && v == least_v;
+      who = __ballot_sync(0xffffffffu, holds);
     }
-    if (top == 0) break;
-    if (best == top && place == top_place) {  // the lane that holds it
+    const Key top_place = __shfl_sync(0xffffffffu, place, __ffs(who) - 1);
+    if (lane == (n & 31)) {
+      const Key top = static_cast<Key>(top_upper) << 32 | top_lower;
+      if (n < 32) { chosen[0] = top; chosen_place[0] = top_place; }
+      else { chosen[1] = top; chosen_place[1] = top_place; }
+    }
+    if (holds) {
       if (comes_to >= 0) sh.list[comes_to].next = coming;
-      const int w = static_cast<int>(top_place >> 32), token = static_cast<int>(static_cast<unsigned>(top_place));
-      a.out_scores[row0 + n] = static_cast<float>(score_of(top));
-      a.parents[row0 + n] = w;
-      a.tokens[row0 + n] = token;
-      a.done[row0 + n] = sh.ended[w] || token == a.end;
       Selection::List& l = sh.list[from];
+      const int w = static_cast<int>(place >> 32);
       offer(l, w, l.next, sh.base[w]);
       coming = l.taken < W ? __ldcg(keys + from * W + l.taken) : 0;
       comes_to = from;
       l.taken += 1;
+      look();
     }
-    __syncwarp();
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int k = half * 32 + lane;
+    if (k >= n) continue;
+    const int w = static_cast<int>(chosen_place[half] >> 32), token = static_cast<int>(static_cast<unsigned>(chosen_place[half]));
+    a.out_scores[row0 + k] = static_cast<float>(score_of(chosen[half]));
+    a.parents[row0 + k] = w;
+    a.tokens[row0 + k] = token;
+    a.done[row0 + k] = sh.ended[w] || token == a.end;
   }
   if (n < W && lane == 0)  // nothing else is left than -inf
     fill_up<T>(logits + row0 * a.vocab, &sh, a.out_scores + row0, a.parents + row0, a.tokens + row0, a.done + row0, n, W, a.vocab, a.end);
@@ -548,10 +576,10 @@ __global__ void __launch_bounds__(32, kWarpsPerSm) beam_step_kernel(const T* __r
 }
 
 // Chunks of a beam, by an estimate in cycles: a warp alone takes 900 for a batch, n on an SM together 82
-// n; a chunk's start and end take 5500; the selection 3000, and for each of W rounds 600 and a look at
+// n; a chunk's start and end take 5500; the selection 3000, and for each of W rounds 450 and a look at
 // all lists.  Chunks that do not fit the device at once cost another round of the same.  (512 rows of
-// 100003: 51 us with 4 or 5 chunks, 57 with 6, 82 with 1; 128 rows of 50021, 16 beams: 37 with 6 to
-// 10, 43 with 16.)
+// 100003: 49 us with 4 or 5 chunks, 55 with 6, 82 with 1; 128 rows of 50021, 16 beams: 33 with 5 to
+// 10, 39 with 16.)
 int choose_chunks(long long rows, int beams, long long vectors, int sms) {
   const double batches = static_cast<double>((vectors + kBatchVectors - 1) / kBatchVectors);
   int best = 1;
@@ -559,7 +587,7 @@ int choose_chunks(long long rows, int beams, long long vectors, int sms) {
   for (int c = 1; c <= batches && c * beams <= kMostLists; ++c) {
     const double tasks = static_cast<double>(rows) * c, beside = std::min<double>(kWarpsPerSm, std::ceil(tasks / sms));
     const double rounds = std::ceil(tasks / (kWarpsPerSm * sms));
-    const double cost = rounds * (std::ceil(batches / c) * std::max(900.0, 82.0 * beside) + 5500.0) + 3000.0 + beams * (600.0 + 1.25 * beams * c);
+    const double cost = rounds * (std::ceil(batches / c) * std::max(900.0, 82.0 * beside) + 5500.0) + 3000.0 + beams * (450.0 + 1.25 * beams * c);
     if (cost < best_cost) { best = c; best_cost = cost; }
   }
   return best;

@@ -6,10 +6,18 @@
 // when interleaved; values behind R and heads behind `rotary_heads` pass through.
 //
 // Bound by memory: every value is read once and written once.  The angles are shared by all heads
-// of a token, so a block takes one token, its first R/2 threads compute that token's sines and
-// cosines once, and the whole block applies them.  The turn count p f_i is formed in float64 (a
-// position of a million times a frequency of one loses 0.06 rad in float32) and reduced to half a
-// turn before it is rounded to float32, which costs three float64 operations per pair and token.
+// of a token, so a block takes one token or a few, forms their sines and cosines once, in shared memory,
+// and applies them to all heads; the heads' values are fetched before and arrive meanwhile.  The turn
+// count p f_i is formed in float64 (a position of a million times a frequency of one loses 0.06 rad in
+// float32) and reduced to half a turn before it is rounded to float32, which costs three float64
+// operations per pair and token.
+//
+// Measured (bfloat16): 8192 tokens of 48 heads of 128, 201 MB read and written in 38 us (5.3 TB/s; a plain
+// copy takes 31).  Without any arithmetic the same structure takes 36: blocks that live for one row leave the
+// memory idle while they start and end.  32768 tokens of 4 heads of 64 take 14 us beyond an empty launch (70
+// with a block for each row or two, 5 by their bytes).  A few rows cost a launch.
+#include <algorithm>
+
 #include "ob/cuda_common.cuh"
 
 namespace ob {
@@ -20,14 +28,15 @@ constexpr int kMaxPairs = 256;
 constexpr int kRotaryThreads = 256;
 
 struct RotaryArgs {
-  long long rows;            // batch * tokens
   long long xs[3], ys[3];    // element strides of batch, token, head
   const void* positions;     // nullptr: the token index
   int positions_64, positions_batched;
+  int rows;                  // batch * tokens
   int tokens, heads, rotary_heads, head_dim, half;
   float sign, magnitude;
   int in_place;
-  unsigned magic_units, magic_tail, magic_wide;  // see quotient()
+  int sets;
+  unsigned magic_units, magic_tail, magic_wide, magic_turned, magic_passed, magic_half, magic_tokens;  // see quotient()
   double turns[kMaxPairs];
 };
 
@@ -36,42 +45,44 @@ struct alignas(sizeof(T) * VEC) Vec {
   T v[VEC];
 };
 
-// n / d by a product with `magic` = ceil(2^32 / d), exact while n d < 2^32; 0: divide.
-__device__ __forceinline__ int quotient(int n, int d, unsigned magic) {
-  return magic != 0 ? static_cast<int>(__umulhi(static_cast<unsigned>(n), magic)) : n / d;
-}
-
-// A block takes TOKENS rows.  Each thread has one unit (VEC pairs of one head) to turn and one access to
-// pass on in each of them; they are fetched first and are under way while the threads look up the
-// positions and form the sines and cosines.  Rows with more units than a block has threads go
-// round again.
-template <class T, int VEC, bool INTER, int TOKENS>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const T* x, T* y, const __grid_constant__ RotaryArgs a) {
+// Rows narrower than a block stand beside each other in `sets` of it; rows with more units (VEC pairs of one
+// head to turn) than the block has threads go round again.  Each thread has one unit to turn and one access to
+// pass on, of one row each; they are fetched first and are under way while the threads look up the
+// positions and form the sines and cosines.
+//
+// Wide rows want the blocks that fit beside each other: 8192 rows of 48 heads of 128 take 38 us with 6 blocks
+// on an SM and 43 with the 5 that the registers would allow; narrow ones gain nothing.  One row at a time:
+// with two for each thread 32768 tokens of 8 heads of 256 take 87 us in place of 77, 4 of 64 23 in place of 19.
+template <class T, int VEC, bool INTER, bool SETS>  // SETS: more than one
+__global__ void __launch_bounds__(kRotaryThreads, SETS ? 1 : 6) rotary_kernel(const T* x, T* y, const __grid_constant__ RotaryArgs a) {
   // `x` may be `y`: each value is read and written by one thread, the read first.
   using V = Vec<T, VEC>;
-  static_assert(TOKENS <= 2, "the table is filled for two rows at most");
   constexpr int PAIRS = INTER ? (VEC + 1) / 2 : VEC;  // of one unit
-  __shared__ float2 table[TOKENS * kMaxPairs];
-  const long long row0 = static_cast<long long>(blockIdx.x) * TOKENS;
-  const int rows = static_cast<int>(min(static_cast<long long>(TOKENS), a.rows - row0));
-  int b = static_cast<int>(row0 / a.tokens), t = static_cast<int>(row0 - static_cast<long long>(b) * a.tokens);
-  const T* xr[TOKENS];
-  T* yr[TOKENS];
-  int token[2];
-#pragma unroll
-  for (int k = 0; k < TOKENS; ++k) {
-    xr[k] = x + (b * a.xs[0] + t * a.xs[1]);
-    yr[k] = y + (b * a.ys[0] + t * a.ys[1]);
-    token[k] = t;
-    if (++t == a.tokens) { t = 0; ++b; }
-  }
-  const int first = blockIdx.y * kRotaryThreads + threadIdx.x, step = gridDim.y * kRotaryThreads;
+  constexpr int kValues = INTER ? 2 * PAIRS : PAIRS;  // of a unit, where it begins
+  extern __shared__ float2 table[];  // of row k, pair j of unit u at k * half + j * units + u: neighbouring threads read neighbouring words
+  const int row0 = blockIdx.x * (SETS ? a.sets : 1), rows = SETS ? min(a.sets, a.rows - row0) : 1;
+  const int b0 = static_cast<unsigned>(row0) / static_cast<unsigned>(a.tokens), t0 = row0 - b0 * a.tokens;
   const int units = a.half / PAIRS, turned = a.rotary_heads * units;  // units to turn in a row
   const int tail = (a.head_dim - 2 * a.half) / VEC, tails = a.rotary_heads * tail, wide = a.head_dim / VEC;
   const int passed = a.in_place ? 0 : tails + (a.heads - a.rotary_heads) * wide;  // accesses to pass on in a row
 
-  // The table holds pair j of unit u at j * units + u: neighbouring threads read neighbouring words.
-  // Offset of unit i; of access i: first the tails of turned heads, then whole heads.
+  // Row k of the block: its sequence and token; where it begins.
+  auto token_of = [&](int k, int* b) {
+    int t = t0 + k;
+    *b = b0;
+    if (SETS && t >= a.tokens) {
+      const int over = quotient(t, a.tokens, a.magic_tokens);
+      *b += over;
+      t -= over * a.tokens;
+    }
+    return t;
+  };
+  auto row_of = [&](auto* data, const long long (&strides)[3], int k) {
+    int b;
+    const int t = token_of(k, &b);
+    return data + (b * strides[0] + t * strides[1]);
+  };
+  // Offset of unit i of a row; of access i: first the tails of turned heads, then whole heads.
   auto unit_at = [&](int i, int* unit) {
     const int h = quotient(i, units, a.magic_units);
     *unit = i - h * units;
@@ -90,11 +101,6 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const T* x, T* y
     *in = h * a.xs[2] + u;
     *out = h * a.ys[2] + u;
   };
-
-  V lo[TOKENS], hi[TOKENS], through[TOKENS];
-  constexpr int kValues = INTER ? 2 * PAIRS : PAIRS;  // of a unit, where it begins
-  int unit = 0;
-  const int head = unit_at(first, &unit), at = unit * kValues;
   auto fetch = [&](const T* row, int h, int u, V* p, V* q) {
     const T* src = row + h * a.xs[2] + u;
     if constexpr (INTER && VEC == 1) {
@@ -105,33 +111,6 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const T* x, T* y
       if constexpr (!INTER) *q = *reinterpret_cast<const V*>(src + a.half);
     }
   };
-  if (first < turned)
-#pragma unroll
-    for (int k = 0; k < TOKENS; ++k)
-      if (k < rows) fetch(xr[k], head, at, &lo[k], &hi[k]);
-  long long in = 0, out = 0;
-  if (first < passed) {
-    access_at(first, &in, &out);
-#pragma unroll
-    for (int k = 0; k < TOKENS; ++k)
-      if (k < rows) through[k] = *reinterpret_cast<const V*>(xr[k] + in);
-  }
-
-  for (int j = threadIdx.x; j < TOKENS * a.half; j += kRotaryThreads) {
-    const int k = TOKENS > 1 && j >= a.half ? 1 : 0, i = j - k * a.half;
-    if (k >= rows) break;
-    const int t_k = TOKENS > 1 && k == 1 ? token[1] : token[0];
-    const long long place = a.positions_batched ? row0 + k : t_k;
-    const double p = a.positions == nullptr ? static_cast<double>(t_k)
-                     : a.positions_64       ? static_cast<double>(static_cast<const long long*>(a.positions)[place])
-                                            : static_cast<double>(static_cast<const int*>(a.positions)[place]);
-    const double u = p * a.turns[i];
-    float s, c;
-    sincospif(2.f * static_cast<float>(u - rint(u)), &s, &c);
-    table[k * kMaxPairs + i % PAIRS * units + i / PAIRS] = make_float2(c * a.magnitude, s * a.magnitude * a.sign);
-  }
-  __syncthreads();
-
   auto turn = [&](T* row, int h, int u, const float2* cs, const V& p, const V& q) {
     T* dst = row + h * a.ys[2] + u;
     if constexpr (INTER && VEC == 1) {
@@ -159,52 +138,82 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const T* x, T* y
       *reinterpret_cast<V*>(dst + a.half) = s;
     }
   };
-  if (first < passed)
-#pragma unroll
-    for (int k = 0; k < TOKENS; ++k)
-      if (k < rows) *reinterpret_cast<V*>(yr[k] + out) = through[k];
-  if (first < turned)
-#pragma unroll
-    for (int k = 0; k < TOKENS; ++k)
-      if (k < rows) turn(yr[k], head, at, table + k * kMaxPairs + unit, lo[k], hi[k]);
+
+  // With several sets a row is no wider than the block: (set, unit) and (set, access) of this thread.
+  // Threads behind the last set belong to no row.
+  int first = blockIdx.y * kRotaryThreads + threadIdx.x, first_pass = first, set = 0, set_pass = 0;
+  const int step = gridDim.y * kRotaryThreads;
+  if constexpr (SETS) {
+    set = quotient(first, turned, a.magic_turned);
+    first -= set * turned;
+    if (passed > 0) {
+      set_pass = quotient(first_pass, passed, a.magic_passed);
+      first_pass -= set_pass * passed;
+    }
+  }
+  const T *xr = row_of(x, a.xs, set), *xp = SETS ? row_of(x, a.xs, set_pass) : xr;
+  T *yr = row_of(y, a.ys, set), *yp = SETS ? row_of(y, a.ys, set_pass) : yr;
+  V lo, hi, through;
+  int unit = 0;
+  const int head = unit_at(first, &unit), at = unit * kValues;
+  const bool turns = first < turned && set < rows, passes = first_pass < passed && set_pass < rows;
+  if (turns) fetch(xr, head, at, &lo, &hi);
+  long long in = 0, out = 0;
+  if (passes) {
+    access_at(first_pass, &in, &out);
+    through = *reinterpret_cast<const V*>(xp + in);
+  }
+  for (int j = threadIdx.x; j < rows * a.half; j += kRotaryThreads) {
+    const int k = !SETS ? 0 : quotient(j, a.half, a.magic_half), i = j - k * a.half;
+    int b;
+    const int t = token_of(k, &b);
+    const long long place = a.positions_batched ? static_cast<long long>(row0) + k : t;
+    const double p = a.positions == nullptr ? static_cast<double>(t)
+                     : a.positions_64       ? static_cast<double>(static_cast<const long long*>(a.positions)[place])
+                                            : static_cast<double>(static_cast<const int*>(a.positions)[place]);
+    const double u = p * a.turns[i];
+    float s, c;
+    sincospif(2.f * static_cast<float>(u - rint(u)), &s, &c);
+    table[k * a.half + i % PAIRS * units + i / PAIRS] = make_float2(c * a.magnitude, s * a.magnitude * a.sign);
+  }
+  __syncthreads();
+  if (passes) *reinterpret_cast<V*>(yp + out) = through;
+  if (turns) turn(yr, head, at, table + set * a.half + unit, lo, hi);
+  if constexpr (SETS) return;
   for (int i = first + step; i < turned; i += step) {
     const int h = unit_at(i, &unit), u = unit * kValues;
-#pragma unroll
-    for (int k = 0; k < TOKENS; ++k)
-      if (k < rows) fetch(xr[k], h, u, &lo[k], &hi[k]);
-#pragma unroll
-    for (int k = 0; k < TOKENS; ++k)
-      if (k < rows) turn(yr[k], h, u, table + k * kMaxPairs + unit, lo[k], hi[k]);
+    fetch(xr, h, u, &lo, &hi);
+    turn(yr, h, u, table + unit, lo, hi);
   }
-  for (int i = first + step; i < passed; i += step) {
+  for (int i = first_pass + step; i < passed; i += step) {
     access_at(i, &in, &out);
-#pragma unroll
-    for (int k = 0; k < TOKENS; ++k)
-      if (k < rows) *reinterpret_cast<V*>(yr[k] + out) = *reinterpret_cast<const V*>(xr[k] + in);
+    *reinterpret_cast<V*>(yr + out) = *reinterpret_cast<const V*>(xr + in);
   }
 }
 
-unsigned magic_of(long long d, long long most) { return d > 1 && most * d < (1ll << 32) ? static_cast<unsigned>(((1ll << 32) + d - 1) / d) : 0u; }
-
 template <class T, int VEC>
 void launch_rotary(const T* x, T* y, RotaryArgs a, bool inter, int sms, cudaStream_t st) {
-  const long long row = static_cast<long long>(a.heads) * a.head_dim;  // accesses of a row and more
-  a.magic_units = magic_of(a.half / (inter ? (VEC + 1) / 2 : VEC), row + 65536);
-  a.magic_tail = magic_of((a.head_dim - 2 * a.half) / VEC, row + 65536);
-  a.magic_wide = magic_of(a.head_dim / VEC, row + 65536);
-  // Enough rows for the device: two to a block.  Few rows leave most SMs without a block: their heads
-  // are spread over several.
-  if (a.rows >= 16ll * sms) {
-    const unsigned grid = static_cast<unsigned>((a.rows + 1) / 2);
-    if (inter) rotary_kernel<T, VEC, true, 2><<<grid, kRotaryThreads, 0, st>>>(x, y, a);
-    else rotary_kernel<T, VEC, false, 2><<<grid, kRotaryThreads, 0, st>>>(x, y, a);
-    return;
-  }
-  long long gy = a.rows >= sms ? 1 : (row / VEC + kRotaryThreads - 1) / kRotaryThreads;
-  if (gy > 64) gy = 64;
-  const dim3 grid(static_cast<unsigned>(a.rows), static_cast<unsigned>(gy < 1 ? 1 : gy));
-  if (inter) rotary_kernel<T, VEC, true, 1><<<grid, kRotaryThreads, 0, st>>>(x, y, a);
-  else rotary_kernel<T, VEC, false, 1><<<grid, kRotaryThreads, 0, st>>>(x, y, a);
+  const long long units = a.half / (inter ? (VEC + 1) / 2 : VEC), turned = a.rotary_heads * units;
+  const long long tail = (a.head_dim - 2 * a.half) / VEC, wide = a.head_dim / VEC, passed = a.in_place ? 0 : a.rotary_heads * tail + (a.heads - a.rotary_heads) * wide;
+  const long long work = std::max(turned, passed);
+  // As many sets as threads have work, while the device keeps several blocks for each SM (8191 rows of 8 heads of
+  // 64, 48 of them turned: 10.3 us with 5 sets, 12.4 with 2, 24 with one; an empty launch about 6).
+  a.sets = static_cast<int>(std::max(1ll, std::min<long long>(kRotaryThreads / work, a.rows / (4ll * sms))));
+  // Few rows leave most SMs without a block: their heads are spread over several.
+  const long long gy = a.rows >= sms ? 1 : std::min(64ll, (work + kRotaryThreads - 1) / kRotaryThreads);
+  const long long most = work + 65536;  // of the indices, and more
+  a.magic_units = magic_of(units, most);
+  a.magic_tail = magic_of(tail, most);
+  a.magic_wide = magic_of(wide, most);
+  a.magic_turned = magic_of(turned, most);
+  a.magic_passed = magic_of(passed, most);
+  a.magic_half = magic_of(a.half, static_cast<long long>(a.sets) * a.half);
+  a.magic_tokens = magic_of(a.tokens, static_cast<long long>(a.tokens) + a.sets);
+  const dim3 grid(static_cast<unsigned>((a.rows + a.sets - 1) / a.sets), static_cast<unsigned>(gy));
+  const size_t smem = static_cast<size_t>(a.sets) * a.half * sizeof(float2);  // half <= VEC work: 16 KB at most
+  auto launch = [&](auto kernel) { kernel<<<grid, kRotaryThreads, smem, st>>>(x, y, a); };
+  if (a.sets > 1) inter ? launch(rotary_kernel<T, VEC, true, true>) : launch(rotary_kernel<T, VEC, false, true>);
+  else inter ? launch(rotary_kernel<T, VEC, true, false>) : launch(rotary_kernel<T, VEC, false, false>);
 }
 
 template <class T>
@@ -213,10 +222,10 @@ void k_rotary(OpCall& c) {
   Tensor& y = c.out[0];
   RotaryArgs a{};
   const long long rows = x.shape()[0] * x.shape()[1];
-  if (rows > 2147483647LL || x.shape()[2] * x.shape()[3] > 2147483647LL)
+  if (rows > 1073741823LL || x.shape()[2] * x.shape()[3] > 1073741823LL)
     throw std::invalid_argument("rotary_embedding: too many tokens or too wide a row");
   const bool inter = c.i[1] != 0;
-  a.rows = rows;
+  a.rows = static_cast<int>(rows);
   a.half = static_cast<int>(turns.numel());
   a.tokens = static_cast<int>(x.shape()[1]);
   a.heads = static_cast<int>(x.shape()[2]);

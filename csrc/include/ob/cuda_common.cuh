@@ -126,6 +126,15 @@ __device__ __forceinline__ bool last_warp_to_arrive(unsigned int* counter, unsig
   return __shfl_sync(0xffffffffu, last, 0) != 0;
 }
 
+// n / d for n, d >= 0 by a product with magic_of(d, most n): `magic` = ceil(2^32 / d) is exact while
+// n d < 2^32; 0: divide.
+__device__ __forceinline__ int quotient(int n, int d, unsigned magic) {
+  return magic != 0 ? static_cast<int>(__umulhi(static_cast<unsigned>(n), magic)) : n / d;
+}
+inline unsigned magic_of(long long d, long long most) {
+  return d > 1 && most < (1ll << 32) / d ? static_cast<unsigned>(((1ll << 32) + d - 1) / d) : 0u;
+}
+
 // Device counter of indices that kernels found out of range (and did not follow).
 unsigned int* index_error_counter();
 

@@ -65,16 +65,6 @@ inline bool extrema_better(T candidate, T best) {
   return candidate > best;
 }
 
-// Beams that offer the same scores tie, whatever order their exponentials were summed in: the
-// logarithm of the sum is rounded to 2^-30, far above the noise of the summation (about 2^-45) and
-// far below what scores are known to (2^-24 of their size).
-#ifdef __CUDACC__
-__host__ __device__
-#endif
-inline double round_log_sum(double log_sum) {
-  return nearbyint(log_sum * 1073741824.0) * (1.0 / 1073741824.0);
-}
-
 // splitmix64 finalizer used by dropout on both backends; element i of a mask uses the
 // top 24 bits of splitmix64(seed + i).  (reference project: src/backends/cpu/unary.cpp:243-267)
 inline uint64_t splitmix64(uint64_t x) {

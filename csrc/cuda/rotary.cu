@@ -50,11 +50,11 @@ struct alignas(sizeof(T) * VEC) Vec {
 // pass on, of one row each; they are fetched first and are under way while the threads look up the
 // positions and form the sines and cosines.
 //
-// Wide rows want the blocks that fit beside each other: 8192 rows of 48 heads of 128 take 38 us with 6 blocks
-// on an SM and 43 with the 5 that the registers would allow; narrow ones gain nothing.  One row at a time:
+// Six blocks on an SM, by a bound on the registers: 8192 rows of 48 heads of 128 take 38 us (43 with the 5 that
+// they would allow), 32768 of 8 heads of 256 75 (91 with 4).  One row at a time:
 // with two for each thread 32768 tokens of 8 heads of 256 take 87 us in place of 77, 4 of 64 23 in place of 19.
 template <class T, int VEC, bool INTER, bool SETS>  // SETS: more than one
-__global__ void __launch_bounds__(kRotaryThreads, SETS ? 1 : 6) rotary_kernel(const T* x, T* y, const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kRotaryThreads, 6) rotary_kernel(const T* x, T* y, const __grid_constant__ RotaryArgs a) {
   // `x` may be `y`: each value is read and written by one thread, the read first.
   using V = Vec<T, VEC>;
   constexpr int PAIRS = INTER ? (VEC + 1) / 2 : VEC;  // of one unit

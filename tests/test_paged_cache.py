@@ -361,3 +361,24 @@ def test_refusals(device):
     assert ob.paged_attention(z(0, 4, 16), kp, vp, i(0, 2), i(0)).shape == (0, 4, 16)
     assert not ob.paged_attention(q, z(0, 2, 8, 16), z(0, 2, 8, 16), i(3, 0), n).cpu().numpy().any()
     ob.paged_append_(kp, vp, z(3, 0, 2, 16), z(3, 0, 2, 16), table, n)
+
+
+@pytest.mark.parametrize("device,dtype", DEVICES)
+@pytest.mark.parametrize("B,T,H,D,P,longest", [(1, 4099, 1, 64, 16, 4099), (3, 1000, 2, 33, 16, 700), (300, 13, 1, 8, 4, 13), (2, 2500, 20, 128, 32, 2500)])
+def test_append_of_many_tokens(device, dtype, B, T, H, D, P, longest):
+    """Tokens that lie beside each other in one block, with counts that end inside it and sequences of no new token."""
+    rng = np.random.default_rng(B + T)
+    starts, counts = rng.integers(0, 40, B), rng.integers(0, longest + 1, B)
+    counts[0], counts[-1] = (T, 0) if B > 1 else (T, T)
+    table, pages = make_table(rng, [int(s) + T for s in starts], P)
+    k, v = (give(rng.standard_normal((B, T, H, D)), dtype, device) for _ in range(2))
+    kp, vp = (give(rng.standard_normal((pages, H, P, D)), dtype, device) for _ in range(2))
+    want = [seen(kp), seen(vp)]
+    for rows, side in zip((seen(k), seen(v)), want):
+        for b in range(B):
+            at = starts[b] + np.arange(counts[b])
+            side[table[b, at // P], :, at % P] = rows[b, :counts[b]]
+    ob.paged_append_(kp, vp, k, v, whole(table, device), whole(starts, device), whole(counts, device))
+    assert np.array_equal(seen(kp), want[0]) and np.array_equal(seen(vp), want[1])
+    if device != "cpu":
+        assert index_errors() == 0

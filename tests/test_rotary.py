@@ -185,3 +185,20 @@ def test_module_holds_the_settings():
     assert np.array_equal(x.numpy(), want.numpy())
     with pytest.raises(ValueError):
         nn.RotaryEmbedding(5)
+
+
+@pytest.mark.parametrize("device,dtype", DEVICES)
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("B,T,H,D,R,heads", [(1, 8191, 1, 32, 32, 1), (4000, 1, 2, 16, 8, 1), (1500, 3, 1, 20, 12, 1), (3, 1999, 8, 64, 48, 8),
+                                             (1, 20011, 5, 8, 8, 1), (700, 5, 1, 33, 2, 1), (2, 1300, 20, 128, 128, 3)])
+def test_many_narrow_rows(device, dtype, inter, B, T, H, D, R, heads):
+    """Rows that lie beside each other in one block: sequences that end inside it, the last block, more to pass on than to turn."""
+    rng = np.random.default_rng(B + T)
+    x, x64 = make(rng, (B, T, H, D), dtype, device)
+    positions = rng.integers(0, 5000, (B, T))
+    p = _C.from_numpy(positions)
+    module = dict(rotary_dim=R, rotary_heads=heads, interleaved=inter)
+    want, size = reference(x64, positions, R, heads, inter)
+    close(ob.rotary_embedding(x, p if device == "cpu" else p.to(device), **module), want, size, dtype)
+    want, size = reference(x64, np.broadcast_to(np.arange(T), (B, T)), R, heads, inter)
+    close(ob.rotary_embedding_(x, **module), want, size, dtype)

@@ -135,6 +135,11 @@ class CausalLM(nn.Module):
         if self.cfg.positions == "learned" and T > self.cfg.max_seq:
             raise ValueError(f"sequence length {T} exceeds max_seq {self.cfg.max_seq}")
 
+    @staticmethod
+    def _check_tokens(tokens, rank, message):
+        if not isinstance(tokens, _C.Tensor) or tokens.ndim != rank or tokens.dtype not in ("int32", "int64"):
+            raise ValueError(message)
+
     def _embed(self, ids):
         x = _C.embedding(ids, self.tok_emb)
         if self.cfg.positions == "rotary":
@@ -167,7 +172,8 @@ class CausalLM(nn.Module):
 
     def prefill(self, ids, cache, sequences, lengths=None):
         """Runs prompts ids [B, T] into empty cache sequences; row b has lengths[b] tokens (default T), padding behind them is
-        ignored.  Returns the logits [B, vocab] of each prompt's last token."""
+        ignored.  Returns the logits [B, vocab] of each prompt's last token.  A call that raises leaves the sequences empty."""
+        self._check_tokens(ids, 2, "prefill: ids must be an int32 or int64 tensor [B, T]")
         B, T = ids.shape
         self._check_length(T)
         lengths = [T] * B if lengths is None else [int(n) for n in lengths]
@@ -177,8 +183,12 @@ class CausalLM(nn.Module):
             raise ValueError("prefill: the sequences must be empty")
         with _no_grad():
             device = str(self.tok_emb.device)
-            cache.extend(sequences, lengths)
-            return self._prefill(ids, cache, cache.table(sequences), _whole([0] * B, device), _whole(lengths, device), lengths)
+            _, before = cache._extend(sequences, lengths)
+            try:
+                return self._prefill(ids, cache, cache.table(sequences), _whole([0] * B, device), _whole(lengths, device), lengths)
+            except BaseException:  # rows that were written already lie behind the sequences' ends
+                cache._take_back(before)
+                raise
 
     def _prefill(self, ids, cache, table, starts, counts, lengths):
         T, E = ids.shape[1], self.cfg.d_model
@@ -192,11 +202,20 @@ class CausalLM(nn.Module):
         return _C.linear(self.ln_f(x), self.head_weight)
 
     def decode(self, tokens, cache, sequences):
-        """One more token of each sequence (int tensor [B]) into the cache.  Returns the logits [B, vocab] behind it."""
+        """One more token of each sequence (int tensor [B]) into the cache.  Returns the logits [B, vocab] behind it.  A call
+        that raises leaves the sequences as they were."""
+        self._check_tokens(tokens, 1, "decode: tokens must be an int32 or int64 tensor [B]")
+        if tokens.shape[0] != len(sequences):
+            raise ValueError(f"decode: {tokens.shape[0]} tokens for {len(sequences)} sequences")
         self._check_length(max([cache.length(s) for s in sequences] + [0]) + 1)
         with _no_grad():
-            places = _whole(cache.extend(sequences, 1), str(self.tok_emb.device))
-            return self._decode(tokens, cache, cache.table(sequences), places, cache.lengths(sequences))
+            starts, before = cache._extend(sequences, 1)
+            try:
+                places = _whole(starts, str(self.tok_emb.device))
+                return self._decode(tokens, cache, cache.table(sequences), places, cache.lengths(sequences))
+            except BaseException:  # rows that were written already lie behind the sequences' ends
+                cache._take_back(before)
+                raise
 
     def _decode(self, tokens, cache, table, places, lengths):
         x = _C.embedding(tokens, self.tok_emb)

@@ -64,6 +64,10 @@ class PagedKVCache:
     def extend(self, sequences, counts):
         """Makes room for `counts` more tokens of each sequence (one number for all, or one each) and counts them as there;
         returns the places where they begin.  Raises, with nothing changed, when the free pages do not suffice."""
+        return self._extend(sequences, counts)[0]
+
+    def _extend(self, sequences, counts):
+        """`extend` that also returns what `_take_back` needs to undo it."""
         sequences = [self._known(s) for s in sequences]
         if len(set(sequences)) != len(sequences):
             raise ValueError("PagedKVCache: a sequence is given twice")
@@ -87,21 +91,41 @@ class PagedKVCache:
         need = sum(private) + sum(fresh)
         if need > len(self._free):
             raise RuntimeError(f"PagedKVCache: out of pages ({need} needed, {len(self._free)} of {self.num_pages} free)")
-        sources, destinations = [], []
+        sources, destinations, before = [], [], []
         for s, start, n, copies, more in zip(sequences, starts, counts, private, fresh):
             pages = self._pages[s]
+            shared = None
             if copies:
                 last = start // self.page_size
                 page = self._take()
-                sources.append(pages[last])
+                shared = pages[last]
+                sources.append(shared)
                 destinations.append(page)
-                self._drop(pages[last])
+                self._drop(shared)
                 pages[last] = page
+            before.append((s, start, len(pages), shared))
             pages.extend(self._take() for _ in range(more))
             self._lengths[s] = start + n
         if sources:
-            copy_pages_(self.pool, sources, destinations, dim=1)
-        return starts
+            try:
+                copy_pages_(self.pool, sources, destinations, dim=1)
+            except BaseException:
+                self._take_back(before)
+                raise
+        return starts, before
+
+    def _take_back(self, before):
+        """Undoes an `_extend` behind which nothing else has happened: lengths, page lists and shared pages as before."""
+        for s, length, count, shared in reversed(before):
+            pages = self._pages[s]
+            while len(pages) > count:
+                self._drop(pages.pop())
+            if shared is not None:
+                last = length // self.page_size
+                self._drop(pages[last])
+                pages[last] = shared
+                self._owners[shared] += 1
+            self._lengths[s] = length
 
     def fork(self, sequence):
         """A new sequence with the same tokens; the pages are shared until one of the two grows."""

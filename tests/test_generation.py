@@ -329,3 +329,79 @@ def test_attention_module_turns_queries_and_keys():
     want = m.out_proj(y.transpose(1, 2).contiguous().reshape([2, 5, 16]))
     assert np.array_equal(m(x, is_causal=True).numpy(), want.numpy())
     assert sorted(m.state_dict()) == sorted(nn.MultiHeadSelfAttention(16, 2).state_dict())
+
+
+# ------------------------------------------------------------- calls that are refused
+def everything(cache):
+    return (dict(cache._lengths), {s: list(p) for s, p in cache._pages.items()}, list(cache._owners), sorted(cache._free))
+
+
+def raises_and_keeps(cache, call, errors):
+    before = everything(cache)
+    with pytest.raises(errors):
+        call()
+    assert everything(cache) == before
+    check_cache(cache)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("more", [{}, ROTARY])
+def test_a_refused_step_leaves_the_cache_as_it_was(device, more):
+    """The next step gives the logits that it gives without the refused ones, bit for bit."""
+    model = build(device, **more)
+    rng = np.random.default_rng(4)
+    ids = rng.integers(0, 97, (2, 8))
+
+    def start():
+        cache = model.new_cache(20, page_size=4)
+        sequences = [cache.add(), cache.add()]
+        model.prefill(whole(ids, device), cache, sequences, [6, 8])
+        sequences.append(cache.fork(sequences[0]))  # a shared page that is not full: the step copies it
+        return cache, sequences
+
+    cache, sequences = start()
+    narrow = nn.PagedKVCache(2, 2, 16, 20, page_size=4, device=device)  # does not fit the model
+    few = nn.PagedKVCache(1, 4, 16, 20, page_size=4, device=device)     # its first layer does
+    for bad in (whole([1], device), whole([1, 2], device), whole([1, 2, 3, 4], device), whole([[1], [2], [3]], device), whole([[1, 2, 3]], device),
+                _C.from_numpy(np.ones(3, np.float32)).to(device), [1, 2, 3], np.array([1, 2, 3])):
+        raises_and_keeps(cache, lambda: model.decode(bad, cache, sequences), ValueError)
+    raises_and_keeps(cache, lambda: model.decode(whole([1, 200, 3], "cpu"), cache, sequences), IndexError)  # host tokens are checked
+    for other, errors in ((narrow, ValueError), (few, IndexError)):
+        fresh = [other.add() for _ in range(2)]
+        raises_and_keeps(other, lambda: model.prefill(whole(ids, device), other, fresh), errors)
+        other.extend(fresh, 3)
+        both = fresh + [other.fork(fresh[0])]
+        raises_and_keeps(other, lambda: model.decode(whole([1, 2, 3], device), other, both), errors)
+    got = model.decode(whole([5, 6, 7], device), cache, sequences).to("cpu").numpy()
+    cache, sequences = start()
+    assert np.array_equal(got, model.decode(whole([5, 6, 7], device), cache, sequences).to("cpu").numpy())
+
+
+def test_a_refused_prompt_leaves_its_sequences_empty():
+    model = build()
+    cache = model.new_cache(6, page_size=4)
+    a, b = cache.add(), cache.add()
+    outside = np.array([[1, 2, 3], [4, 97, 6]])
+    raises_and_keeps(cache, lambda: model.prefill(whole(outside, "cpu"), cache, [a, b]), IndexError)
+    raises_and_keeps(cache, lambda: model.prefill(whole([1, 2, 3], "cpu"), cache, [a]), ValueError)
+    raises_and_keeps(cache, lambda: model.prefill(_C.from_numpy(np.ones((1, 3), np.float32)), cache, [a]), ValueError)
+    raises_and_keeps(cache, lambda: model.prefill(whole(np.ones((2, 16)), "cpu"), cache, [a, b]), RuntimeError)  # out of pages
+    assert cache.free_pages == 6
+    got = model.prefill(whole(outside % 97, "cpu"), cache, [a, b]).numpy()
+    cache = model.new_cache(6, page_size=4)
+    assert np.array_equal(got, model.prefill(whole(outside % 97, "cpu"), cache, [cache.add(), cache.add()]).numpy())
+
+
+def test_an_interrupted_copy_leaves_the_cache_as_it_was(monkeypatch):
+    from orthon_b200.nn import kv_cache
+
+    cache = nn.PagedKVCache(1, 1, 4, 8, page_size=4)
+    a = cache.add()
+    cache.extend([a], 6)
+    b = cache.fork(a)
+
+    def fails(*args, **kw):
+        raise RuntimeError("no copy")
+
+    monkeypatch.setattr(kv_cache, "copy_pages_", fails)
+    raises_and_keeps(cache, lambda: cache.extend([a, b], [5, 1]), RuntimeError)

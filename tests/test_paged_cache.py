@@ -382,3 +382,29 @@ def test_append_of_many_tokens(device, dtype, B, T, H, D, P, longest):
     assert np.array_equal(seen(kp), want[0]) and np.array_equal(seen(vp), want[1])
     if device != "cpu":
         assert index_errors() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("room", [0, 5000])
+@pytest.mark.parametrize("H,K,D", [(8, 4, 64), (24, 2, 128), (6, 6, 96)])
+def test_weights_keep_more_bits_than_the_cache(dtype, room, H, K, D):
+    """One value of each query and key is not zero, so a score is a product and no sum: off by 2^-24 of itself for each of three
+    roundings (scale, base, difference to the maximum), and its weight by that, twice (own and sum), and 2^-21 for exp2 and the
+    running rescaling.  Two terms of the type, the first rounded down (a step) and the second to the nearest (half a step of what
+    is left), hold a weight to 2 half steps^2.  With the sums of n < 100 weights and
+    products, (n + 2) 2^-24 each, that is far below half a step of the weights; what is left is half a step of the output."""
+    rng, lengths, P = np.random.default_rng(H + D), [48, 31, 64, 96], 16
+    table, pages = make_table(rng, lengths, P)
+    table = np.pad(table, ((0, 0), (0, max(0, -(-room // P) - table.shape[1]))))
+    raw = np.zeros((2, pages, K, P, D))
+    raw[0, ..., 5] = rng.uniform(-2, 2, (pages, K, P))
+    raw[1] = rng.standard_normal((pages, K, P, D))
+    queries = np.zeros((len(lengths), H, D))
+    queries[..., 5] = rng.uniform(0.5, 1.5, (len(lengths), H))
+    q, kp, vp = (give(x, dtype, "cuda:0") for x in (queries, raw[0], raw[1]))
+    got = seen(ob.paged_attention(q, kp, vp, whole(table, "cuda:0"), whole(lengths, "cuda:0"), scale=1.0))
+    want, size, spread = attend(seen(q), seen(kp), seen(vp), table, lengths, 1.0)
+    weight = 2 * 3 * 2.0 ** -24 * 2 * spread[..., None] + 2.0 ** -21 + 2 * HALF_STEP[dtype] ** 2 + 2 * (max(lengths) + 2) * 2.0 ** -24
+    bad = ~(abs(got - want) <= weight * size + abs(want) * HALF_STEP[dtype] * 1.001 + TINY[dtype])
+    assert not bad.any(), (int(bad.sum()), bad.size, float(abs(got - want).max()))

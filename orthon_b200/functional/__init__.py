@@ -74,7 +74,7 @@ def _rotary_frequencies(rotary_dim, base, scaling):
     f_i = base^(-2i/R).  'linear' divides every frequency by the factor; 'ntk' enlarges the base so that the slowest pair is
     stretched by the factor and the fastest not at all; 'yarn' (Peng et al., 2023) stretches pairs that turn less than
     beta_slow times over the original length, leaves those that turn more than beta_fast times, ramps in between, and
-    enlarges queries and keys by 0.1 ln(factor) + 1."""
+    enlarges queries and keys by 0.1 ln(factor) + 1 (not at all for a factor below 1)."""
     kind, factor, original, fast, slow, attention = scaling or (None, 1.0, 1.0, 32.0, 1.0, None)
     if kind == "ntk":
         if rotary_dim <= 2:
@@ -93,7 +93,7 @@ def _rotary_frequencies(rotary_dim, base, scaling):
     span = high - low if high > low else 0.001
     ramp = [min(1.0, _builtins.max(0.0, (i - low) / span)) for i in range(rotary_dim // 2)]
     mixed = [f * (1.0 - r) + f / factor * r for f, r in zip(plain, ramp)]
-    return mixed, 0.1 * _math.log(factor) + 1.0 if attention is None else attention
+    return mixed, 0.1 * _math.log(_builtins.max(factor, 1.0)) + 1.0 if attention is None else attention
 
 
 @_lru_cache(maxsize=256)

@@ -202,3 +202,20 @@ def test_many_narrow_rows(device, dtype, inter, B, T, H, D, R, heads):
     close(ob.rotary_embedding(x, p if device == "cpu" else p.to(device), **module), want, size, dtype)
     want, size = reference(x64, np.broadcast_to(np.arange(T), (B, T)), R, heads, inter)
     close(ob.rotary_embedding_(x, **module), want, size, dtype)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("factor", [0.5, 1e-6, 1.0])
+def test_yarn_does_not_shrink_below_a_factor_of_one(device, factor):
+    """The enlargement is 0.1 ln(factor) + 1 from a factor of 1 on, and 1 below: turned pairs keep their length.  Their length is
+    off by the rounding of two products, a sum, sine and cosine (2^-22 in all) and of the results (2^-24 each)."""
+    rng = np.random.default_rng(7)
+    x = rng.standard_normal((2, 5, 2, 8)).astype(np.float32)
+    scaling = {"type": "yarn", "factor": factor, "original_length": 64}
+    give = lambda s: ob.rotary_embedding(_C.from_numpy(x).to(device), scaling=s).to("cpu").numpy().astype(np.float64)  # noqa: E731
+    y = give(scaling)
+    size = lambda a: np.hypot(a[..., :4], a[..., 4:])  # noqa: E731
+    want = size(x.astype(np.float64))
+    assert (abs(size(y) - want) <= want * 2.0 ** -21).all()
+    assert np.array_equal(give({**scaling, "attention_factor": 1.0}), y)
+    assert not np.array_equal(give({**scaling, "attention_factor": 0.75}), y)

@@ -55,7 +55,7 @@ def _rotary_scaling(scaling):
     allowed = {"factor"} | ({"original_length", "beta_fast", "beta_slow", "attention_factor"} if kind == "yarn" else set())
     if set(rest) - allowed:
         raise ValueError(f"rotary scaling '{kind}' does not take {sorted(set(rest) - allowed)}")
-    if "factor" not in rest or (kind == "yarn" and "original_length" not in rest):
+    if rest.get("factor") is None or (kind == "yarn" and rest.get("original_length") is None):
         raise ValueError(f"rotary scaling '{kind}' needs " + ("'factor' and 'original_length'" if kind == "yarn" else "'factor'"))
     values = {"original_length": 1.0, "beta_fast": 32.0, "beta_slow": 1.0, **{k: v for k, v in rest.items() if v is not None}}
     for name, value in values.items():

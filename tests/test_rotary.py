@@ -219,3 +219,10 @@ def test_yarn_does_not_shrink_below_a_factor_of_one(device, factor):
     assert (abs(size(y) - want) <= want * 2.0 ** -21).all()
     assert np.array_equal(give({**scaling, "attention_factor": 1.0}), y)
     assert not np.array_equal(give({**scaling, "attention_factor": 0.75}), y)
+
+
+@pytest.mark.parametrize("scaling", [{"type": "linear", "factor": None}, {"type": "yarn", "factor": None, "original_length": 8},
+                                     {"type": "yarn", "factor": 2.0, "original_length": None}])
+def test_a_scaling_without_its_numbers_is_refused(scaling):
+    with pytest.raises(ValueError, match="needs"):
+        ob.rotary_embedding(ob.zeros([1, 2, 1, 4]), scaling=scaling)

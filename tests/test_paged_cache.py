@@ -408,3 +408,20 @@ def test_weights_keep_more_bits_than_the_cache(dtype, room, H, K, D):
     weight = 2 * 3 * 2.0 ** -24 * 2 * spread[..., None] + 2.0 ** -21 + 2 * HALF_STEP[dtype] ** 2 + 2 * (max(lengths) + 2) * 2.0 ** -24
     bad = ~(abs(got - want) <= weight * size + abs(want) * HALF_STEP[dtype] * 1.001 + TINY[dtype])
     assert not bad.any(), (int(bad.sum()), bad.size, float(abs(got - want).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("B,at,long,H,K,D", [(700, 0, 30000, 2, 1, 64), (600, 599, 40001, 3, 1, 40), (300, 150, 20000, 8, 2, 128), (1100, 7, 70000, 1, 1, 128)])
+def test_one_sequence_far_longer_than_the_rest(dtype, B, at, long, H, K, D):
+    """Its many shares are joined by more than one warp."""
+    rng = np.random.default_rng(B)
+    lengths = [int(n) for n in rng.integers(0, 40, B)]
+    lengths[at], lengths[(at + 1) % B] = long, long // 3
+    table, pages = make_table(rng, lengths, 16)
+    q = give(rng.standard_normal((B, H, D)) * 2, dtype, "cuda:0")
+    kp, vp = (give(rng.standard_normal((pages, K, 16, D), dtype=np.float32), dtype, "cuda:0") for _ in range(2))
+    args = q, kp, vp, whole(table, "cuda:0"), whole(lengths, "cuda:0")
+    got = ob.paged_attention(*args)
+    check_attention(got, seen(q), seen(kp), seen(vp), table, lengths, D ** -0.5, dtype)
+    assert np.array_equal(seen(got), seen(ob.paged_attention(*args)))

@@ -24,6 +24,7 @@
 // lanes by their place in the row, exponentials are summed with compensation (to about 2^-45, so
 // that their order hardly matters either), and the sum is rounded to float32 before its logarithm.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "ob/cuda_common.cuh"
@@ -32,7 +33,7 @@ namespace ob {
 namespace cu {
 namespace {
 
-constexpr int kWarpsPerSm = 19, kMostLists = 256;  // blocks of one warp; chunks of a sentence that the selection has room for
+constexpr int kWarpsPerSm = 19, kMostLists = 256;  // blocks of one warp, at most; chunks of a sentence that the selection has room for
 constexpr int kBatch = 4, kBatchVectors = kBatch * 32, kRing = 3, kStageBytes = (kBatchVectors + 1) * 16;
 constexpr int kAside = kBatchVectors + 32;  // pieces that a warp has room for: at least a batch at any time
 using Key = unsigned long long;  // order-preserving image of the value, then the complement of its place
@@ -576,21 +577,36 @@ __global__ void __launch_bounds__(32, kWarpsPerSm) beam_step_kernel(const T* __r
 }
 
 // Chunks of a beam, by an estimate in cycles: a warp alone takes 900 for a batch, n on an SM together 82
-// n; a chunk's start and end take 5500; the selection 3000, and for each of W rounds 450 and a look at
-// all lists.  Chunks that do not fit the device at once cost another round of the same.  (512 rows of
-// 100003: 49 us with 4 or 5 chunks, 55 with 6, 82 with 1; 128 rows of 50021, 16 beams: 33 with 5 to
-// 10, 39 with 16.)
-int choose_chunks(long long rows, int beams, long long vectors, int sms) {
+// n; a chunk's start and end take 5500, and from 8 beams on more, as its lists grow; the selection 3000, and for each
+// of W rounds 450 and a look at all lists.  Chunks that do not fit the device at once cost another round of the same.
+// (512 rows of 100003: 46 us with 4 or 5 chunks, 55 with 6, 82 with 1; 128 rows of 50021, 16 beams: 32 with 5 to
+// 10, 39 with 16.  Over 54 sizes of 4 to 64 beams and 1 to 192 sentences the choice takes 1.026 times the best one's time;
+// with 19 blocks on an SM and 5500 for every number of beams it took 1.044, 1.37 at worst.)
+int choose_chunks(long long rows, int beams, long long vectors, int sms, int per_sm) {
   const double batches = static_cast<double>((vectors + kBatchVectors - 1) / kBatchVectors);
+  const double ends = 5500.0 * std::max(1.0, beams / 8.0);
   int best = 1;
   double best_cost = 1e300;
   for (int c = 1; c <= batches && c * beams <= kMostLists; ++c) {
-    const double tasks = static_cast<double>(rows) * c, beside = std::min<double>(kWarpsPerSm, std::ceil(tasks / sms));
-    const double rounds = std::ceil(tasks / (kWarpsPerSm * sms));
-    const double cost = rounds * (std::ceil(batches / c) * std::max(900.0, 82.0 * beside) + 5500.0) + 3000.0 + beams * (450.0 + 1.25 * beams * c);
+    const double tasks = static_cast<double>(rows) * c, beside = std::min<double>(per_sm, std::ceil(tasks / sms));
+    const double rounds = std::ceil(tasks / (static_cast<double>(per_sm) * sms));
+    const double cost = rounds * (std::ceil(batches / c) * std::max(900.0, 82.0 * beside) + ends) + 3000.0 + beams * (450.0 + 1.25 * beams * c);
     if (cost < best_cost) { best = c; best_cost = cost; }
   }
   return best;
+}
+
+// Resident blocks per SM: 19 with lists of 128 keys (up to 8 beams), 17 with 256, 15 with 512.
+template <class T>
+int blocks_on_sm(int room, size_t smem) {
+  static std::atomic<int> known[3];
+  int n = known[room].load(std::memory_order_relaxed);
+  if (n == 0) {
+    OB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, beam_step_kernel<T>, 32, smem));
+    if (n < 1) throw std::runtime_error("beam_search_step: the kernel does not fit this device");
+    known[room].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 template <class T>
@@ -598,7 +614,9 @@ void k_beam_step(OpCall& c) {
   const Shape& s = c.in[0].shape();
   constexpr int N = Values<T>::N;
   const long long rows = s[0] * s[1], vectors = (s[2] + N - 1) / N;
-  const long long chunks = choose_chunks(rows, static_cast<int>(s[1]), vectors, sm_count_for(c.in[0]));
+  const int room = s[1] <= 8 ? 0 : s[1] <= 16 ? 1 : 2, list = 128 << room;
+  const size_t smem = warp_bytes(list);
+  const long long chunks = choose_chunks(rows, static_cast<int>(s[1]), vectors, sm_count_for(c.in[0]), blocks_on_sm<T>(room, smem));
   if (rows * chunks > 2147483647LL) throw std::invalid_argument("beam_search_step: too many rows");
   BeamArgs a{};
   a.scores = c.in[1].data_as<float>();
@@ -621,8 +639,7 @@ void k_beam_step(OpCall& c) {
   a.keys = reinterpret_cast<Key*>(static_cast<char*>(scratch.data()) + stat_bytes);
   const T* logits = c.in[0].data_as<T>();
   a.arrived = arrival_counters(c.in[0].device(), st, static_cast<size_t>(s[0]));
-  a.list = s[1] <= 8 ? 128 : s[1] <= 16 ? 256 : 512;
-  const size_t smem = warp_bytes(a.list);
+  a.list = list;
   static_assert(sizeof(Selection) <= warp_bytes(128), "the selection lies in the chunk's memory");
   beam_step_kernel<T><<<static_cast<unsigned>(rows * chunks), 32, smem, st>>>(logits, a);
   check_launch("beam_search_step");

@@ -20,9 +20,12 @@
 // taken one by one.  Values of -inf are no candidates; the selection is filled up with them if
 // nothing else is left.
 //
-// Beams that offer equal scores have to tie, at whatever address their rows begin: values belong to
-// lanes by their place in the row, exponentials are summed with compensation (to about 2^-45, so
-// that their order hardly matters either), and the sum is rounded to float32 before its logarithm.
+// Beams of the same logits have to tie, at whatever address their rows begin: values belong to lanes by their
+// place in the row, so that the same numbers are added in the same order.  The same logits in another order need not
+// tie: an exponential (2^-22 of itself) is taken relative to the largest logit so far, and a new largest one rescales
+// the sum by a rounded factor, so that the order matters at about 2^-22 of the sum.  The sum itself is compensated: the
+// thousands of additions of a lane would lose more than that.  Candidates of different beams are told apart down to
+// the error of their lse, 2^-20 at most in the tests; those of one beam by their logits, exactly.
 #include <algorithm>
 #include <atomic>
 #include <cmath>

@@ -129,3 +129,62 @@ def test_strided_logits_and_refusals(device):
         ob.beam_search_step(z(2, 3, 50).requires_grad_(), z(2, 3))
     with pytest.raises(ob.UnsupportedOperation):
         ob.beam_search_step(z(2, 3, 50, d="int32"), z(2, 3))
+
+
+@pytest.mark.parametrize("device,dtype", DEVICES)
+@pytest.mark.parametrize("V", [300, 9000, 50021])
+def test_the_same_logits_in_another_order(device, dtype, V):
+    """Beams whose logits are those of another one in another order, the largest first, last, or anywhere.  The CPU, whose sums
+    hardly depend on the order, ties them; CUDA tells them apart by no more than twice the error of a log-sum (2^-20 each)."""
+    rng = np.random.default_rng(V)
+    rows = np.sort(rng.standard_normal((3, 1, V)) * 3, -1) * np.ones((1, 6, 1))
+    rows[:, 1] = rows[:, 1, ::-1]
+    for b in range(3):
+        for w in (2, 3, 4):
+            rows[b, w] = rng.permutation(rows[b, w])
+    rows[:, 5] = rows[:, 4]                                       # and one in the same order
+    scores = np.zeros((3, 6)) - 1.0
+    if device == "cpu":
+        check(rows, scores, None, None, dtype, device)
+    x = give(rows, dtype, device)
+    got = [seen(t) for t in ob.beam_search_step(x, give(scores, "float32", device))]
+    values = seen(x).astype(np.float64)
+    lse = np.log(np.sort(np.exp(values - values.max(-1, keepdims=True)), -1).sum(-1, keepdims=True)) + values.max(-1, keepdims=True)
+    cand = scores[..., None] + (values - lse)
+    best = -np.sort(-cand.reshape(3, -1), -1)[:, :6]
+    off = 2.0 ** -20 + abs(best) * 2.0 ** -24
+    assert (abs(got[0] - best) <= 2 * off).all()
+    for b in range(3):
+        places = list(zip(got[1][b], got[2][b]))
+        assert len(set(places)) == 6
+        assert (abs(np.array([cand[b, w, v] for w, v in places]) - got[0][b]) <= off[b]).all()
+        tokens = {w: [v for u, v in places if u == w] for w in (4, 5)}
+        assert tokens[5] == tokens[4][: len(tokens[5])]           # beam 5 offers what beam 4 does, behind it
+
+
+@pytest.mark.parametrize("device,dtype", DEVICES)
+def test_many_sentences_and_calls_of_different_sizes(device, dtype):
+    """Few and many sentences in turn, more than a first call makes room for."""
+    rng = np.random.default_rng(11)
+    for B, W, V in ((3, 2, 40), (5000, 2, 9), (1, 8, 5000), (4097, 1, 33), (9000, 3, 8), (2, 3, 30001), (5000, 2, 9)):
+        check(rng.standard_normal((B, W, V)) * 3, -rng.random((B, W)), rng.random((B, W)) < 0.2, V - 1, dtype, device)
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once():
+    import threading
+
+    rng, failed = np.random.default_rng(12), []
+    work = [(rng.standard_normal(s) * 3, -rng.random(s[:2])) for s in ((6000, 2, 17), (3, 8, 20001), (64, 4, 999), (12000, 1, 50))]
+
+    def run(logits, scores):
+        try:
+            for _ in range(5):
+                check(logits, scores, None, 3, "float32", "cuda:0")
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed, failed

@@ -425,3 +425,15 @@ def test_one_sequence_far_longer_than_the_rest(dtype, B, at, long, H, K, D):
     got = ob.paged_attention(*args)
     check_attention(got, seen(q), seen(kp), seen(vp), table, lengths, D ** -0.5, dtype)
     assert np.array_equal(seen(got), seen(ob.paged_attention(*args)))
+
+
+@pytest.mark.parametrize("device", PLACES)
+@pytest.mark.parametrize("pairs", [439, 440, 441, 508, 509, 510, 1018, 1019])
+def test_lists_of_copies_at_the_ends_of_a_launch(device, pairs):
+    rng = np.random.default_rng(pairs)
+    a = rng.integers(0, 1000, (2, 2 * pairs + 3, 5)).astype(np.int32)
+    order = rng.permutation(2 * pairs + 3)
+    t = give(a, "int32", device)
+    ob.copy_pages_(t, order[:pairs].tolist(), order[pairs:2 * pairs].tolist(), dim=1)
+    a[:, order[pairs:2 * pairs]] = a[:, order[:pairs]]
+    assert np.array_equal(t.to("cpu").numpy(), a)

@@ -144,15 +144,15 @@ void k_paged_append(OpCall& c) {
 }
 
 // ------------------------------------------------------------------ page copies
-// The pairs travel in the launch's parameters, as many as fit 4 KB: no list is sent to the device first.  1.2 GB
-// read and written take 185 us (6.5 TB/s, as a plain copy); a few pages a launch.
-constexpr int kParameterBytes = 4096, kPairs = (kParameterBytes - 3 * 8) / 8;
+// The pairs travel in the launch's parameters: no list is sent to the device first.  4 KB would hold 509 of them, but a
+// launch with all of 4 KB takes 5.6 us in place of 5.0, and most calls have a few pairs.  1.2 GB read and written
+// take 185 us (6.5 TB/s, as a plain copy); a few pages a launch.
+constexpr int kPairs = 440;
 struct CopyArgs {
   char* base;
   long long page_units, outer_units;  // one page; all pages of one outer index
   int2 pair[kPairs];                  // (source, destination)
 };
-static_assert(sizeof(CopyArgs) <= kParameterBytes, "the pairs fill what is left of the parameters");
 
 template <class U>
 __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ CopyArgs a) {

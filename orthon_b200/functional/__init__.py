@@ -103,15 +103,19 @@ def _rotary_plan(rotary_dim, base, scaling):
     return _C.from_numpy(_np.asarray(radians, dtype=_np.float64) / (2.0 * _np.pi)), magnitude
 
 
+def _checked_rotary_plan(rotary_dim, base, scaling):
+    if not (float(base) > 1.0 and _math.isfinite(float(base))):
+        raise ValueError("rotary base must be finite and larger than 1")
+    return _rotary_plan(rotary_dim, float(base), _rotary_scaling(scaling))
+
+
 def _rotary_call(native, x, positions, rotary_dim, rotary_heads, base, interleaved, scaling, transposed):
     if x.ndim != 4:
         raise ValueError("rotary_embedding expects input with shape [B, T, H, D]")
     rotary_dim = int(x.shape[3] if rotary_dim is None else rotary_dim)
     if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > x.shape[3]:
         raise ValueError(f"rotary_dim must be even and in [2, {x.shape[3]}], got {rotary_dim}")
-    if not (float(base) > 1.0 and _math.isfinite(float(base))):
-        raise ValueError("rotary base must be finite and larger than 1")
-    turns, magnitude = _rotary_plan(rotary_dim, float(base), _rotary_scaling(scaling))
+    turns, magnitude = _checked_rotary_plan(rotary_dim, base, scaling)
     return native(x, positions, turns, magnitude, int(x.shape[2] if rotary_heads is None else rotary_heads), bool(interleaved), bool(transposed))
 
 

@@ -69,6 +69,8 @@ class Block(nn.Module):
         if cfg.positions == "rotary":
             self.rotary = nn.RotaryEmbedding(self.head_dim if cfg.rotary_dim is None else cfg.rotary_dim, base=cfg.rotary_base,
                                              interleaved=cfg.rotary_interleaved, scaling=cfg.rotary_scaling)
+            if self.rotary.rotary_dim > self.head_dim:
+                raise ValueError(f"rotary_dim {self.rotary.rotary_dim} exceeds the head size {self.head_dim}")
         self.scale = 1.0 / math.sqrt(E // cfg.n_heads)
         self.ln1 = nn.LayerNorm(E, eps=cfg.eps)
         self.qkv_weight, self.qkv_bias = _normal((E, 3 * E), cfg.init_std), nn.Parameter(_C.zeros([3 * E]))

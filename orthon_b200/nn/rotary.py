@@ -1,5 +1,5 @@
 """Rotary positions as a module: a configuration without parameters or buffers."""
-from ..functional import rotary_embedding, rotary_embedding_
+from ..functional import _checked_rotary_plan, rotary_embedding, rotary_embedding_
 from .module import Module
 
 
@@ -13,8 +13,9 @@ class RotaryEmbedding(Module):
         super().__init__()
         self.rotary_dim, self.base, self.interleaved = int(rotary_dim), float(base), bool(interleaved)
         self.scaling = None if scaling is None else dict(scaling)
-        if self.rotary_dim < 2 or self.rotary_dim % 2:
-            raise ValueError("rotary_dim must be even and at least 2")
+        if not 2 <= self.rotary_dim <= 512 or self.rotary_dim % 2:
+            raise ValueError("rotary_dim must be even and in [2, 512]")
+        _checked_rotary_plan(self.rotary_dim, self.base, self.scaling)
 
     def _settings(self):
         return dict(rotary_dim=self.rotary_dim, base=self.base, interleaved=self.interleaved, scaling=self.scaling)

@@ -405,3 +405,21 @@ def test_an_interrupted_copy_leaves_the_cache_as_it_was(monkeypatch):
 
     monkeypatch.setattr(kv_cache, "copy_pages_", fails)
     raises_and_keeps(cache, lambda: cache.extend([a, b], [5, 1]), RuntimeError)
+
+
+@pytest.mark.parametrize("bad", [dict(rotary_dim=18), dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_base=1.0), dict(rotary_base=float("nan")),
+                                 dict(rotary_scaling={"type": "other", "factor": 2.0}), dict(rotary_scaling={"type": "yarn", "factor": 2.0}),
+                                 dict(rotary_dim=2, rotary_scaling={"type": "ntk", "factor": 2.0})])
+def test_rotary_settings_are_refused_when_the_model_is_built(bad):
+    with pytest.raises(ValueError):
+        build(positions="rotary", **bad)
+    settings = {k.replace("rotary_", ""): v for k, v in bad.items() if k != "rotary_dim"}
+    if bad.get("rotary_dim") != 18:
+        with pytest.raises(ValueError):
+            nn.RotaryEmbedding(bad.get("rotary_dim", 16), **settings)
+
+
+def test_a_module_takes_the_sizes_that_the_operator_takes():
+    nn.RotaryEmbedding(512)
+    with pytest.raises(ValueError):
+        nn.RotaryEmbedding(514)

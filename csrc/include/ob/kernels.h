@@ -49,8 +49,6 @@
 //  BeamSearchStep     in0=logits[B,W,V] in1=scores f32[B,W] in2=finished bool[B,W]? out0=scores f32 out1=parents i64
 //                     out2=tokens i64 out3=finished bool (all [B,W]) i0=end token (-1: none)
 #pragma once
-#include <math.h>
-
 #include "ob/dispatch.h"
 
 namespace ob {

@@ -236,8 +236,8 @@ class CausalLM(nn.Module):
         steps, W = int(max_new_tokens), int(num_beams)
         if len(lengths) != B or any(not 1 <= n <= T for n in lengths):
             raise ValueError("generate: one length in [1, T] for each prompt")
-        if steps < 0 or W < 1:
-            raise ValueError("generate: max_new_tokens must not be negative and num_beams at least 1")
+        if steps < 0 or W < 1 or int(page_size) < 1:
+            raise ValueError("generate: max_new_tokens must not be negative, num_beams and page_size at least 1")
         if eos_token is not None and not 0 <= int(eos_token) < self.cfg.vocab_size:
             raise ValueError("generate: eos_token is not in the vocabulary")
         self._check_length(max([T] + [n + steps for n in lengths]))

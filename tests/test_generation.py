@@ -423,3 +423,10 @@ def test_a_module_takes_the_sizes_that_the_operator_takes():
     nn.RotaryEmbedding(512)
     with pytest.raises(ValueError):
         nn.RotaryEmbedding(514)
+
+
+@pytest.mark.parametrize("more", [{}, dict(num_beams=2)])
+@pytest.mark.parametrize("page_size", [0, -4])
+def test_generation_refuses_pages_without_room(more, page_size):
+    with pytest.raises(ValueError, match="page_size"):
+        build().generate(whole(np.zeros((2, 3)), "cpu"), 3, page_size=page_size, **more)

@@ -170,6 +170,8 @@ def beam_search_step(logits, scores, finished=None, eos_token=None):
     token.  ``parents`` and ``tokens`` (int64) tell the beam and the token of each; a beam is finished with its parent or with
     ``eos_token``.  A beam whose score is not finite, or whose logits have a NaN or +inf or are all -inf, offers nothing:
     its continuations count as -inf."""
+    if eos_token is not None and int(eos_token) < 0:
+        raise IndexError("beam_search_step: the end token is out of range")
     return _C._beam_search_step(logits, scores, finished, -1 if eos_token is None else int(eos_token))
 
 

@@ -188,3 +188,10 @@ def test_two_threads_at_once():
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert not failed, failed
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda:0", marks=pytest.mark.gpu)])
+def test_a_negative_end_token_is_refused(device):
+    """-1, by which the kernels know that there is none, is no exception."""
+    with pytest.raises(IndexError):
+        ob.beam_search_step(give(np.zeros((1, 2, 5)), "float32", device), give(np.zeros((1, 2)), "float32", device), eos_token=-1)

@@ -146,7 +146,10 @@ class PagedKVCache:
         sequences = [self._known(s) for s in sequences]
         if len(set(sequences)) != len(sequences):
             raise ValueError("PagedKVCache: a sequence is given twice")
-        chosen = [sequences[int(p)] for p in parents]
+        parents = [int(p) for p in parents]
+        if any(not 0 <= p < len(sequences) for p in parents):
+            raise IndexError("PagedKVCache: a parent is out of range")
+        chosen = [sequences[p] for p in parents]
         new = [self.fork(s) for s in chosen]
         for s in sequences:
             self.free(s)

@@ -430,3 +430,11 @@ def test_a_module_takes_the_sizes_that_the_operator_takes():
 def test_generation_refuses_pages_without_room(more, page_size):
     with pytest.raises(ValueError, match="page_size"):
         build().generate(whole(np.zeros((2, 3)), "cpu"), 3, page_size=page_size, **more)
+
+
+@pytest.mark.parametrize("parents", [[0, -1], [2, 0]])
+def test_parents_are_places_in_the_list(parents):
+    cache = nn.PagedKVCache(1, 1, 4, 4, page_size=2)
+    sequences = [cache.add(), cache.add()]
+    cache.extend(sequences, [3, 1])
+    raises_and_keeps(cache, lambda: cache.reorder(sequences, parents), IndexError)

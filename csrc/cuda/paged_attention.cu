@@ -528,7 +528,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_tile_kernel(const __grid_
       // The weights enter the product with the values as two terms of the cache's type, 15 (bfloat16) or 21 bits of
       // them: the output is as near as with float32 weights.  One term, that is weights rounded by half a step beside a
       // sum that is not, was off by 0.0021 of the output in bfloat16, two are by 0.0017, which is the output's own
-      // rounding; they take 62.1 us in place of 59.9 for 32 ragged sequences of up to 4096 tokens with 32 heads on 8.
+      // rounding; they take 99.3 us in place of 98.7 for 131072 tokens with 32 heads on 8, and a block with a head of
+      // its own 11.5 in place of 10.3 for 512 tokens.
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         split2(s[nt][2 * e], s[nt][2 * e + 1], &p[nt][e], &p2[nt][e], static_cast<T*>(nullptr));
@@ -1018,15 +1019,17 @@ void launch_own(Kernel kernel, int threads, size_t smem, const PagedArgs& a, con
   check_launch("paged_attention");
 }
 
-// A block per head, or even shares and a second kernel?  The second kernel costs about 7 us; a block alone
-// takes 0.0094 us for a token of 512 bytes, until 1.6 heads on each SM keep the memory busy.  Lengths
-// are on the device: what the table has room for stands for them, and a table beyond 4096 tokens,
-// where one long sequence could keep a few blocks running alone, gets even shares.  (Own against
-// shares, 8 cached heads of 128: 1 sequence of 512 tokens 10.3 / 13.7 us, 1024 14.5 / 14.3, 2048 24.7 /
-// 16.4; 16 of up to 2048 26.5 / 32.8; 64 of up to 2048 58.7 / 67.5; 8 of 8192 84.4 / 58.4.)
-bool block_per_head(const PagedArgs& a, int sms) {
-  const double room = static_cast<double>(a.table_width) * a.page_size, heads = static_cast<double>(a.batch) * a.kv_heads * a.tiles;
-  return room <= 4096.0 && (1.0 - heads / (1.6 * sms)) * room <= 1000.0;
+// A block per head, or even shares and a second kernel?  The second kernel costs 7 to 10 us.  A block alone takes
+// `per_token` us for a token of its head (bfloat16: 0.009, 0.011 and 0.015 with 64, 128 and 256 values; float32: 0.03 to
+// 0.055), until 1.2 heads on each SM keep the device busy.  Lengths are on the device: what the table has room for
+// stands for them, and a table where one long sequence could keep a few blocks running alone for over 25 us gets even
+// shares.  (Own against shares, bfloat16, 8 cached heads of 128, 4 query heads on each: 1 sequence of 512 tokens 11.5 / 12.4
+// us, 1024 17.0 / 13.4, 2048 28.8 / 13.4; 16 of up to 2048 29.3 / 34.4; 64 of up to 2048 58.8 / 66.3; 32 of up to 4096
+// 61.8 / 59.1; 8 of 8192 98.6 / 61.0.  float32: 32 of up to 1000, 4 heads of 64 42.6 / 28.8.  Over 220 sizes of both types
+// the choice takes 1.009 times the better one's time, 1.32 at worst; without any block per head it would be 1.23.)
+bool block_per_head(const PagedArgs& a, int sms, double per_token) {
+  const double alone = per_token * a.table_width * a.page_size, heads = static_cast<double>(a.batch) * a.kv_heads * a.tiles;
+  return alone <= 25.0 && (1.0 - heads / (1.2 * sms)) * alone <= 10.0;
 }
 
 template <class T, int KD, int NT, int STAGES, int WARPS, int OWN_STAGES>
@@ -1035,14 +1038,14 @@ void launch_tiles(PagedArgs a, const Launch& l) {
   a.tiles = (group + most - 1) / most;
   a.tile_heads = (group + a.tiles - 1) / a.tiles;
   constexpr size_t slab = 2 * SlabLayout<KD>::kBytes;
-  if (block_per_head(a, l.sms)) launch_own(paged_tile_kernel<T, KD, NT, OWN_STAGES, 4, true>, 128, 4 * OWN_STAGES * slab, a, l);
+  if (block_per_head(a, l.sms, 0.0075 + 0.00003 * a.head_dim)) launch_own(paged_tile_kernel<T, KD, NT, OWN_STAGES, 4, true>, 128, 4 * OWN_STAGES * slab, a, l);
   else launch_both<T>(paged_tile_kernel<T, KD, NT, STAGES, WARPS, false>, WARPS * 32, WARPS * STAGES * slab, a, l);
 }
 
 template <class T, int PER, int NH>
 void launch_rows(const PagedArgs& a, const Launch& l, bool wide) {
   constexpr size_t own = kRowThreads / 32 * static_cast<size_t>(NH) * (PER * 32 * sizeof(float) + sizeof(float2));  // for every head size of the kernel
-  if (block_per_head(a, l.sms)) launch_own(paged_rows_kernel<T, PER, NH, true>, kRowThreads, own, a, l, wide);
+  if (block_per_head(a, l.sms, 0.025 + 0.003 * a.tile_heads + 0.00004 * a.head_dim)) launch_own(paged_rows_kernel<T, PER, NH, true>, kRowThreads, own, a, l, wide);
   else launch_both<T>(paged_rows_kernel<T, PER, NH, false>, kRowThreads, 0, a, l, wide);
 }
 

@@ -3,9 +3,11 @@
 //   candidate (w, v) = score_w + x_wv - lse_w,   lse_w = log sum_v exp x_wv
 //
 // The logits are read once; that is the floor (512 rows of 100003 in bfloat16, every fifth at its end:
-// 82 MB, 12.5 us).  It takes 46 us: a batch of 1024 logits costs a warp about 330 instructions, of
-// which exponentials and their compensated sum are half, and 11 warps on an SM get through one in
-// 150 cycles; the start of a warp, with cold code, and the selection are 10 us.  Within a beam the order of the candidates is the
+// 82 MB, 12.5 us).  It takes 46 us.  A batch of 1024 logits costs a warp about 330 instructions, of which exponentials and
+// their compensated sum are half: the 40000 batches are 13 of the 17.5 million that are issued, 16 us if every slot
+// were taken.  Half are: a scheduler has 2.3 warps on average, each with one batch at a time, and the SMs are active for 52 to 84
+// thousand cycles, since blocks of finished beams leave at once and the others fall on SMs by chance.  The start
+// of a warp, with cold code, and the selection are 10 us.  Within a beam the order of the candidates is the
 // order of the logits, so the beams are cut into chunks, and a warp takes from one its W best (value,
 // lowest place) together with its maximum and sum of exponentials, in one pass.  The last warp of a
 // sentence to arrive forms each beam's lse and picks the W best of the chunks' winners, in float64.

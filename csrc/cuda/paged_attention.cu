@@ -12,7 +12,9 @@
 // within one warp's share is written at once; one that is spread leaves (m, sum p, sum p v) of each
 // share in a workspace, and a second kernel joins them in order.  No atomics: the same call gives the
 // same bits.  (Joining inside the first kernel, by the last warp to arrive, was measured too: 116 us
-// instead of 99 for 131072 tokens, because its fences wait for the streams around it.)
+// instead of 99 for 131072 tokens, because its fences wait for the streams around it.)  Even shares are even in
+// slabs: heads of one slab take longer for it, for their queries and outputs are waited for (a call that is
+// waited for, 8 cached heads of 128: one sequence of 131072 tokens 133 us, beside 255 of one token 232).
 //
 // Short caches are not worth a second kernel, and many heads need no division: there a block takes
 // one head of one sequence, its warps every slab in turn, and they join in shared memory.
@@ -1068,7 +1070,8 @@ void attend(const PagedArgs& a, const Launch& l) {
   if constexpr (sizeof(T) == 2) {
     if (a.head_dim % 8 == 0 && strides % 8 == 0 && bases % 16 == 0) {
       // Up to 8 query heads of a cached head fill one product; more warps where a slab is short: it takes
-      // a warp about as long whatever its bytes (128 sequences of up to 2000, 16 heads of 64: 16 warps 96 us).
+      // a warp about as long whatever its bytes (128 sequences of up to 4000, 16 heads of 64: 182 us with
+      // 16 warps, 212 with 8).
       const bool one = a.heads / a.kv_heads <= 8;
       if (a.head_dim <= 64) one ? launch_tiles<T, 4, 1, 3, 16, 4>(a, l) : launch_tiles<T, 4, 2, 6, 8, 4>(a, l);
       else if (a.head_dim <= 96) one ? launch_tiles<T, 6, 1, 2, 12, 3>(a, l) : launch_tiles<T, 6, 2, 4, 8, 3>(a, l);

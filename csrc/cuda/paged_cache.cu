@@ -30,9 +30,11 @@ struct AppendArgs {
 // kAhead for each thread.  The first kAhead of a thread are fetched at once, while other threads look up
 // the tokens' places.  The bound on registers keeps 6 blocks on an SM.
 //
-// Measured (bfloat16): 8192 tokens of 8 heads of 128, keys and values, 67 MB in 14.5 us (16.5 with the 4 blocks
-// that the registers would allow; 39 with one token to a block); 32768 tokens of 2 heads of 64 12 us (129); an
-// empty launch takes about 6.  One token of each sequence costs a launch.
+// Measured, calls one after another (bfloat16): 8192 tokens of 8 heads of 128, keys and values, 67 MB in 15.5 us (16.6
+// with the blocks that the registers would allow; 38 with one token to a block); 32768 tokens of 2 heads of 64 10.4 us
+// (127).  8 padded prompts of up to 1024 tokens of 16 heads of 128, 72 MB: 16.5 us, 11.0 by their bytes; 2212 of the 4096
+// blocks have rows and 888 fit the device, so that these are two and a half waves of blocks that look a place
+// up, load once and store once.  One token of each sequence costs a launch.
 template <class U>
 __global__ void __launch_bounds__(kThreads, 6) append_kernel(const __grid_constant__ AppendArgs a) {
   __shared__ long long to[kThreads];  // first access of a token's place, -1: not written

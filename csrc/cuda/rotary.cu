@@ -10,12 +10,15 @@
 // and applies them to all heads; the heads' values are fetched before and arrive meanwhile.  The turn
 // count p f_i is formed in float64 (a position of a million times a frequency of one loses 0.06 rad in
 // float32) and reduced to half a turn before it is rounded to float32, which costs three float64
-// operations per pair and token.
+// operations per pair and token.  From there on float32: a float32 result is off by 5.7e-8 of its size, where sines
+// and cosines in float64 would leave 4.2e-8; 16-bit results are the same.
 //
-// Measured (bfloat16): 8192 tokens of 48 heads of 128, 201 MB read and written in 38 us (5.3 TB/s; a plain
-// copy takes 31).  Without any arithmetic the same structure takes 36: blocks that live for one row leave the
-// memory idle while they start and end.  32768 tokens of 4 heads of 64 take 14 us beyond an empty launch (70
-// with a block for each row or two, 5 by their bytes).  A few rows cost a launch.
+// Measured, calls one after another (bfloat16): 8192 tokens of 48 heads of 128, 201 MB read and written in 39 us
+// (5.1 TB/s; a plain copy takes 31).  Without any arithmetic the same structure takes 36: blocks that live for one row
+// leave the memory idle while they start and end.  32768 tokens of 4 heads of 64: 18.6 us (66 with a block for each row;
+// 5 by their bytes).  float32, 8191 tokens of 8 heads of 64, neighbouring pairs, 48 values turned: 12.3 us for 33.5 MB
+// (5.1): 70 % of the issue slots are taken, 247 instructions for each warp, which moves 16 or 32 bytes a lane; they are places,
+// divisions of the index and the angles.  A few rows cost a call, 4.7 us, of which the launch is most.
 #include <algorithm>
 
 #include "ob/cuda_common.cuh"
@@ -50,8 +53,8 @@ struct alignas(sizeof(T) * VEC) Vec {
 // pass on, of one row each; they are fetched first and are under way while the threads look up the
 // positions and form the sines and cosines.
 //
-// Six blocks on an SM, by a bound on the registers: 8192 rows of 48 heads of 128 take 38 us (43 with the 5 that
-// they would allow), 32768 of 8 heads of 256 75 (91 with 4).  One row at a time:
+// Six blocks on an SM, by a bound on the registers: 8192 rows of 48 heads of 128 take 39 us (46 with what
+// they would allow), 32768 of 8 heads of 256 76 (82).  One row at a time:
 // with two for each thread 32768 tokens of 8 heads of 256 take 87 us in place of 77, 4 of 64 23 in place of 19.
 template <class T, int VEC, bool INTER, bool SETS>  // SETS: more than one
 __global__ void __launch_bounds__(kRotaryThreads, 6) rotary_kernel(const T* x, T* y, const __grid_constant__ RotaryArgs a) {
@@ -197,7 +200,7 @@ void launch_rotary(const T* x, T* y, RotaryArgs a, bool inter, int sms, cudaStre
   const long long tail = (a.head_dim - 2 * a.half) / VEC, wide = a.head_dim / VEC, passed = a.in_place ? 0 : a.rotary_heads * tail + (a.heads - a.rotary_heads) * wide;
   const long long work = std::max(turned, passed);
   // As many sets as threads have work, while the device keeps several blocks for each SM (8191 rows of 8 heads of
-  // 64, 48 of them turned: 10.3 us with 5 sets, 12.4 with 2, 24 with one; an empty launch about 6).
+  // 64 in float32: 10.4 us with 4 sets, 12.5 with 2, 16.5 with one).
   a.sets = static_cast<int>(std::max(1ll, std::min<long long>(kRotaryThreads / work, a.rows / (4ll * sms))));
   // Few rows leave most SMs without a block: their heads are spread over several.
   const long long gy = a.rows >= sms ? 1 : std::min(64ll, (work + kRotaryThreads - 1) / kRotaryThreads);
